@@ -324,6 +324,94 @@ int mg_interpolate_force_gather(int on);
 int mg_narrow(const double* src, float* dst, size_t n, void* stream);
 int mg_widen(const float* src, double* dst, size_t n, void* stream);
 
+/* ---- learned type vectors ------------------------------------------------
+ * No counterpart in the reference, whose type vectors are one-hot rows
+ * (CoordinateSet::make_vector_types, src/coordinateset.cpp) or come from a typer:
+ * these entry points make the vectors that mg_forward_vector takes out of type
+ * indices and a table that is learned, and take mg_backward_vector's
+ * type_gradients back to the table.
+ *
+ * Element types (`dtype`): arrays of that type are computed with in float and
+ * rounded once, to the nearest, where they are stored.  `param_dtype` is
+ * MG_FLOAT32 or equal to dtype.  Index kinds: a float index counts as the whole
+ * number below it, as in mg_forward_index; an index below 0, at or beyond nrows,
+ * or not-a-number names no row.  Array pointers are aligned to their elements
+ * (MG_ERR_INVALID_ARGUMENT otherwise), workspaces to 256 bytes. */
+enum { MG_FLOAT32 = 0, MG_FLOAT16 = 1, MG_BFLOAT16 = 2 };
+enum { MG_INDEX_FLOAT32 = 0, MG_INDEX_INT32 = 1, MG_INDEX_INT64 = 2 };
+
+/* out[n,:] = s_n * table[type_index[n],:], a row of zeros where the index names
+ * no row.  s_n = scales[n], or `scale` for every token when scales is NULL.
+ *   type_index [ntokens], table [nrows, channels], scales [ntokens] float32,
+ *   out [ntokens, channels] */
+int mg_embed_types(int ntokens, int nrows, int channels, int dtype, int index_kind,
+                   const void* type_index, const void* table, float scale, const float* scales,
+                   void* out, void* stream);
+
+/* Gradients of mg_embed_types for the upstream gradient `grad`
+ * [ntokens, channels]:
+ *   grad_table [nrows, channels]: sum of s_n * grad[n,:] over the tokens of a row, in float and
+ *     in an order that the sizes and indices alone decide (the same call gives the same bits);
+ *     rows without tokens get zero
+ *   grad_scales [ntokens] float32: sum over the channels of grad[n,:] * table[type_index[n],:]
+ * Either may be NULL; `table` is read for grad_scales only. */
+size_t mg_embed_types_backward_workspace_size(int ntokens, int nrows, int channels);
+int mg_embed_types_backward(int ntokens, int nrows, int channels, int dtype, int index_kind,
+                            const void* type_index, const void* grad, const void* table,
+                            float scale, const float* scales, void* grad_table,
+                            float* grad_scales, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* out = (x - mean) * rstd * weight + bias over the channels of every row, with
+ * rstd = 1 / sqrt(variance + eps).  weight and bias may be NULL (ones, zeros);
+ * mean and rstd [nrows] float32 are what the backward pass takes and may both be
+ * NULL.  out == x is allowed. */
+int mg_layer_norm(int nrows, int channels, int dtype, int param_dtype, const void* x,
+                  const void* weight, const void* bias, float eps, void* out, float* mean,
+                  float* rstd, void* stream);
+
+/* Gradients of mg_layer_norm: grad_x [nrows, channels], grad_weight and
+ * grad_bias [channels] of param_dtype, each of which may be NULL.  The sums over
+ * the rows are float, in an order that the sizes alone decide.  grad_x == grad
+ * is not allowed. */
+size_t mg_layer_norm_backward_workspace_size(int nrows, int channels);
+int mg_layer_norm_backward(int nrows, int channels, int dtype, int param_dtype, const void* grad,
+                           const void* x, const float* mean, const float* rstd,
+                           const void* weight, void* grad_x, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[e] = in[e] * 65536 / (65536 - T) where element e is kept, 0 (whatever in[e]
+ * is) where it is dropped, T = round(65536 p): p is a multiple of 1/65536 and the
+ * expectation of out is in exactly.  Element e is kept where its 16 random bits
+ * are at least T: half e % 8 (the low half of a word first) of the four words that
+ * Philox4x32 with ten rounds gives for the counter (e / 8, offset) and the key
+ * seed.  The mask is stored nowhere: the backward pass is the same call on the
+ * gradient.  `state` (device, two uint64: seed, offset) replaces the two numbers
+ * when it is not NULL, for graphs that are replayed with other numbers.
+ * out == in is allowed. */
+int mg_dropout(uint64_t n, int dtype, const void* in, double p, uint64_t seed, uint64_t offset,
+               const uint64_t* state, void* out, void* stream);
+
+/* out = dropout(layer_norm(scale * table[type_index])), rounded once; element
+ * (n, c) has the position n * channels + c in the dropout.  A row of zeros where
+ * the index names no row. */
+int mg_encode_types(int ntokens, int nrows, int channels, int dtype, int param_dtype,
+                    int index_kind, const void* type_index, const void* table, float scale,
+                    const void* weight, const void* bias, float eps, double p, uint64_t seed,
+                    uint64_t offset, const uint64_t* state, void* out, void* stream);
+
+/* Gradients of mg_encode_types: grad_table [nrows, channels], grad_weight and
+ * grad_bias [channels]; each may be NULL.  All tokens of a row share its
+ * normed vector and the norm's backward pass is linear in the gradient, so the
+ * gradients of a row's tokens are summed first (float, fixed order). */
+size_t mg_encode_types_backward_workspace_size(int ntokens, int nrows, int channels);
+int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, int param_dtype,
+                             int index_kind, const void* type_index, const void* grad,
+                             const void* table, float scale, const void* weight, float eps,
+                             double p, uint64_t seed, uint64_t offset, const uint64_t* state,
+                             void* grad_table, void* grad_weight, void* grad_bias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,10 @@ from .grid_io import *  # noqa: F401,F403,E402
 from .torch_bindings import (BatchedCoords2GridFunction, Coords2Grid, Coords2GridFunction,  # noqa: F401,E402
                              Grid2CoordsGradientFunction, MolIterDataset, MolMapDataset,
                              make_grid_ndarray, make_grid_tensor, tensor_as_grid)
+from .type_vectors import (TypeDropout, TypeDropoutFunction, TypeEmbedding, TypeEmbeddingFunction,  # noqa: F401,E402
+                           TypeEncoder, TypeEncoderFunction, TypeNorm, TypeNormFunction, dropout,
+                           embed_types, embed_types_backward, encode_types, encode_types_backward,
+                           layer_norm, layer_norm_backward)
 
 GridMaker.make_tensor = make_grid_tensor
 GridMaker.make_ndarray = make_grid_ndarray

@@ -15,6 +15,8 @@ MG_ERR_OUT_OF_RANGE = -2
 MG_ERR_UNSUPPORTED = -3
 MG_ERR_NULL_POINTER = -4
 MG_STATIC_SCRATCH_BYTES = 16 << 20
+MG_FLOAT32, MG_FLOAT16, MG_BFLOAT16 = 0, 1, 2
+MG_INDEX_FLOAT32, MG_INDEX_INT32, MG_INDEX_INT64 = 0, 1, 2
 
 EXPORTED_SYMBOLS = (
     "mg_version", "mg_error_string", "mg_trace_ranges", "mg_gridmaker_init", "mg_transform_forward",
@@ -26,6 +28,10 @@ EXPORTED_SYMBOLS = (
     "mg_backward_index_unrotated",
     "mg_backward_vector", "mg_backward_relevance", "mg_backward_gradients", "mg_interpolate", "mg_interpolate_force_gather",
     "mg_narrow", "mg_widen",
+    "mg_embed_types", "mg_embed_types_backward", "mg_embed_types_backward_workspace_size",
+    "mg_layer_norm", "mg_layer_norm_backward", "mg_layer_norm_backward_workspace_size",
+    "mg_dropout", "mg_encode_types", "mg_encode_types_backward",
+    "mg_encode_types_backward_workspace_size",
 )
 
 
@@ -101,10 +107,22 @@ def declare(lib):
     lib.mg_forward_index_paged.argtypes = [_i]
     lib.mg_forward_index_core_skip.argtypes = [_i]
     lib.mg_trace_ranges.argtypes = [_i]
+    size, u64, f64 = ctypes.c_size_t, ctypes.c_uint64, ctypes.c_double
+    lib.mg_embed_types.argtypes = [_i] * 5 + [_vp, _vp, _f, _vp, _vp, _vp]
+    lib.mg_embed_types_backward.argtypes = [_i] * 5 + [_vp] * 3 + [_f] + [_vp] * 4 + [size, _vp]
+    lib.mg_layer_norm.argtypes = [_i] * 4 + [_vp] * 3 + [_f] + [_vp] * 4
+    lib.mg_layer_norm_backward.argtypes = [_i] * 4 + [_vp] * 9 + [size, _vp]
+    lib.mg_dropout.argtypes = [u64, _i, _vp, f64, u64, u64, _vp, _vp, _vp]
+    lib.mg_encode_types.argtypes = [_i] * 6 + [_vp, _vp, _f, _vp, _vp, _f, f64, u64, u64] + [_vp] * 3
+    lib.mg_encode_types_backward.argtypes = ([_i] * 6 + [_vp] * 3 + [_f, _vp, _f, f64, u64, u64] +
+                                             [_vp] * 5 + [size, _vp])
+    for name in ("mg_embed_types_backward_workspace_size", "mg_layer_norm_backward_workspace_size",
+                 "mg_encode_types_backward_workspace_size"):
+        getattr(lib, name).argtypes = [_i] * (2 if "layer_norm" in name else 3)
+        getattr(lib, name).restype = size
     for name in EXPORTED_SYMBOLS:
         fn = getattr(lib, name)
-        if name not in ("mg_error_string", "mg_forward_index_workspace_size",
-                        "mg_forward_vector_workspace_size"):
+        if name != "mg_error_string" and not name.endswith("_workspace_size"):
             fn.restype = _i
     return lib
 

@@ -14,7 +14,7 @@ LIB_NAME = "libmolgrid_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["capi.hip", "transform.hip", "convert.hip", "forward_sorted.hip", "forward_vector.hip", "forward_vector_mfma.hip",
-           "backward.hip", "second_order.hip", "interpolate.hip"]
+           "backward.hip", "second_order.hip", "interpolate.hip", "embed.hip", "layer_norm.hip", "dropout.hip"]
 
 # Packed FP32 instructions are kept out of the generated code.
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

@@ -81,6 +81,43 @@ int check_common(const mg_gridmaker* g, int nbatch, const int32_t* offsets, int 
 
 int from_hip(hipError_t e) { return e == hipSuccess ? MG_OK : (int)e; }
 
+// Arguments of the learned type vectors' entry points.
+bool is_dtype(int dtype) { return dtype >= MG_FLOAT32 && dtype <= MG_BFLOAT16; }
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+size_t dtype_size(int dtype) { return dtype == MG_FLOAT32 ? 4 : 2; }
+size_t index_size(int kind) { return kind == MG_INDEX_INT64 ? 8 : 4; }
+
+int check_tokens(const TokenArg& t) {
+  if (t.ntokens < 0 || t.nrows < 0 || t.channels < 0) return MG_ERR_INVALID_ARGUMENT;
+  if (!is_dtype(t.dtype)) return MG_ERR_INVALID_ARGUMENT;
+  if (t.index_kind < MG_INDEX_FLOAT32 || t.index_kind > MG_INDEX_INT64) return MG_ERR_INVALID_ARGUMENT;
+  if (!aligned(t.index, index_size(t.index_kind))) return MG_ERR_INVALID_ARGUMENT;
+  return MG_OK;
+}
+int check_norm(const NormArg& a) {
+  if (a.nrows < 0 || a.channels < 0) return MG_ERR_INVALID_ARGUMENT;
+  if (!is_dtype(a.dtype) || (a.param_dtype != MG_FLOAT32 && a.param_dtype != a.dtype))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (!(a.eps >= 0.f)) return MG_ERR_INVALID_ARGUMENT;
+  if (!aligned(a.weight, dtype_size(a.param_dtype))) return MG_ERR_INVALID_ARGUMENT;
+  return MG_OK;
+}
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need == 0) return MG_OK;
+  if (workspace == nullptr) return MG_ERR_NULL_POINTER;
+  return !aligned(workspace, 256) || bytes < need ? MG_ERR_INVALID_ARGUMENT : MG_OK;
+}
+int drop_arg(double p, uint64_t seed, uint64_t offset, const uint64_t* state, DropArg* drop) {
+  if (!(p >= 0.0 && p <= 1.0)) return MG_ERR_INVALID_ARGUMENT;   // (also where p is not a number)
+  if (!aligned(state, 8)) return MG_ERR_INVALID_ARGUMENT;
+  drop->limit = (uint32_t)std::floor(p * 65536.0 + 0.5);
+  drop->factor = drop->limit < 65536u ? (float)(65536.0 / (65536 - (int)drop->limit)) : 0.f;
+  drop->seed = seed;
+  drop->offset = offset;
+  drop->state = state;
+  return MG_OK;
+}
+
 // Optional roctx ranges around the entry points (mg_trace_ranges): the marker library is looked up
 // at run time, so the library does not depend on it.
 typedef int (*RangePush)(const char*);
@@ -624,5 +661,188 @@ int mg_interpolate(float in_resolution, float in_dimension, float out_resolution
 }
 
 int mg_interpolate_force_gather(int on) { return mg::set_interpolate_force_gather(on); }
+
+int mg_embed_types(int ntokens, int nrows, int channels, int dtype, int index_kind,
+                   const void* type_index, const void* table, float scale, const float* scales,
+                   void* out, void* stream) {
+  const Range range("mg_embed_types");
+  const TokenArg t{type_index, ntokens, nrows, channels, dtype, index_kind};
+  int rc = check_tokens(t);
+  if (rc != MG_OK) return rc;
+  if (!aligned(table, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) || !aligned(scales, 4))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (ntokens == 0 || channels == 0) return MG_OK;
+  if (type_index == nullptr || out == nullptr || (table == nullptr && nrows > 0))
+    return MG_ERR_NULL_POINTER;
+  return from_hip(launch_embed(t, table, scale, scales, out, (hipStream_t)stream));
+}
+
+size_t mg_embed_types_backward_workspace_size(int ntokens, int nrows, int channels) {
+  if (ntokens <= 0 || nrows <= 0 || channels <= 0) return 0;
+  return row_sums_workspace_bytes(ntokens, nrows, channels);
+}
+
+int mg_embed_types_backward(int ntokens, int nrows, int channels, int dtype, int index_kind,
+                            const void* type_index, const void* grad, const void* table,
+                            float scale, const float* scales, void* grad_table,
+                            float* grad_scales, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  const Range range("mg_embed_types_backward");
+  const TokenArg t{type_index, ntokens, nrows, channels, dtype, index_kind};
+  int rc = check_tokens(t);
+  if (rc != MG_OK) return rc;
+  const size_t size = dtype_size(dtype);
+  if (!aligned(grad, size) || !aligned(table, size) || !aligned(scales, 4) ||
+      !aligned(grad_table, size) || !aligned(grad_scales, 4))
+    return MG_ERR_INVALID_ARGUMENT;
+  const bool to_table = grad_table != nullptr && nrows > 0 && channels > 0;
+  const bool to_scales = grad_scales != nullptr && ntokens > 0;
+  if (ntokens > 0 && channels > 0 && (to_table || to_scales) &&
+      (type_index == nullptr || grad == nullptr))
+    return MG_ERR_NULL_POINTER;
+  if (to_scales && nrows > 0 && channels > 0 && table == nullptr) return MG_ERR_NULL_POINTER;
+  if (to_table) {
+    rc = check_workspace(workspace, workspace_bytes,
+                         mg_embed_types_backward_workspace_size(ntokens, nrows, channels));
+    if (rc != MG_OK) return rc;
+    rc = from_hip(launch_embed_backward(t, grad, scale, scales, grad_table, workspace,
+                                        workspace_bytes, (hipStream_t)stream));
+    if (rc != MG_OK) return rc;
+  }
+  if (to_scales)
+    rc = from_hip(launch_scale_gradient(t, grad, table, grad_scales, (hipStream_t)stream));
+  return rc;
+}
+
+int mg_layer_norm(int nrows, int channels, int dtype, int param_dtype, const void* x,
+                  const void* weight, const void* bias, float eps, void* out, float* mean,
+                  float* rstd, void* stream) {
+  const Range range("mg_layer_norm");
+  const NormArg a{nrows, channels, dtype, param_dtype, weight, eps};
+  const int rc = check_norm(a);
+  if (rc != MG_OK) return rc;
+  if (!aligned(x, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) ||
+      !aligned(bias, dtype_size(param_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (nrows == 0 || channels == 0) return MG_OK;
+  if (x == nullptr || out == nullptr || (mean == nullptr) != (rstd == nullptr))
+    return MG_ERR_NULL_POINTER;
+  return from_hip(launch_norm(a, x, bias, out, mean, rstd, (hipStream_t)stream));
+}
+
+size_t mg_layer_norm_backward_workspace_size(int nrows, int channels) {
+  if (nrows <= 0 || channels <= 0) return 0;
+  return norm_backward_workspace_bytes(nrows, channels);
+}
+
+int mg_layer_norm_backward(int nrows, int channels, int dtype, int param_dtype, const void* grad,
+                           const void* x, const float* mean, const float* rstd,
+                           const void* weight, void* grad_x, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  const Range range("mg_layer_norm_backward");
+  const NormArg a{nrows, channels, dtype, param_dtype, weight, 0.f};
+  int rc = check_norm(a);
+  if (rc != MG_OK) return rc;
+  const size_t size = dtype_size(dtype), param_size = dtype_size(param_dtype);
+  if (!aligned(grad, size) || !aligned(x, size) || !aligned(grad_x, size) || !aligned(mean, 4) ||
+      !aligned(rstd, 4) || !aligned(grad_weight, param_size) || !aligned(grad_bias, param_size))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (grad_x != nullptr && (grad_x == grad || grad_x == x)) return MG_ERR_INVALID_ARGUMENT;
+  const bool any = grad_x != nullptr || grad_weight != nullptr || grad_bias != nullptr;
+  if (channels == 0 || !any) return MG_OK;
+  if (nrows > 0 && (grad == nullptr || x == nullptr || mean == nullptr || rstd == nullptr))
+    return MG_ERR_NULL_POINTER;
+  if (grad_weight != nullptr || grad_bias != nullptr) {
+    rc = check_workspace(workspace, workspace_bytes,
+                         mg_layer_norm_backward_workspace_size(nrows, channels));
+    if (rc != MG_OK) return rc;
+  }
+  return from_hip(launch_norm_backward(a, grad, x, mean, rstd, grad_x, grad_weight, grad_bias,
+                                       workspace, (hipStream_t)stream));
+}
+
+int mg_dropout(uint64_t n, int dtype, const void* in, double p, uint64_t seed, uint64_t offset,
+               const uint64_t* state, void* out, void* stream) {
+  const Range range("mg_dropout");
+  if (!is_dtype(dtype)) return MG_ERR_INVALID_ARGUMENT;
+  DropArg drop;
+  const int rc = drop_arg(p, seed, offset, state, &drop);
+  if (rc != MG_OK) return rc;
+  if (!aligned(in, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (n == 0) return MG_OK;
+  if (n > ((uint64_t)1 << 48)) return MG_ERR_OUT_OF_RANGE;
+  if (in == nullptr || out == nullptr) return MG_ERR_NULL_POINTER;
+  return from_hip(launch_dropout(in, (size_t)n, dtype, drop, out, (hipStream_t)stream));
+}
+
+int mg_encode_types(int ntokens, int nrows, int channels, int dtype, int param_dtype,
+                    int index_kind, const void* type_index, const void* table, float scale,
+                    const void* weight, const void* bias, float eps, double p, uint64_t seed,
+                    uint64_t offset, const uint64_t* state, void* out, void* stream) {
+  const Range range("mg_encode_types");
+  const TokenArg t{type_index, ntokens, nrows, channels, dtype, index_kind};
+  const NormArg a{nrows, channels, dtype, param_dtype, weight, eps};
+  DropArg drop;
+  int rc = check_tokens(t);
+  if (rc == MG_OK) rc = check_norm(a);
+  if (rc == MG_OK) rc = drop_arg(p, seed, offset, state, &drop);
+  if (rc != MG_OK) return rc;
+  if (!aligned(table, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) ||
+      !aligned(bias, dtype_size(param_dtype)))
+    return MG_ERR_INVALID_ARGUMENT;
+  if (ntokens == 0 || channels == 0) return MG_OK;
+  if (type_index == nullptr || out == nullptr || (table == nullptr && nrows > 0))
+    return MG_ERR_NULL_POINTER;
+  return from_hip(launch_encode(t, a, table, scale, bias, drop, out, (hipStream_t)stream));
+}
+
+// The sums over every row's tokens come first in the workspace, then what either step needs.
+size_t mg_encode_types_backward_workspace_size(int ntokens, int nrows, int channels) {
+  if (nrows <= 0 || channels <= 0) return 0;
+  const size_t sums = ((size_t)nrows * channels * sizeof(float) + 255) / 256 * 256;
+  const size_t tokens = ntokens > 0 ? row_sums_workspace_bytes(ntokens, nrows, channels) : 0;
+  const size_t norm = norm_backward_workspace_bytes(nrows, channels);
+  return sums + (tokens > norm ? tokens : norm);
+}
+
+int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, int param_dtype,
+                             int index_kind, const void* type_index, const void* grad,
+                             const void* table, float scale, const void* weight, float eps,
+                             double p, uint64_t seed, uint64_t offset, const uint64_t* state,
+                             void* grad_table, void* grad_weight, void* grad_bias,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  const Range range("mg_encode_types_backward");
+  const TokenArg t{type_index, ntokens, nrows, channels, dtype, index_kind};
+  const NormArg a{nrows, channels, dtype, param_dtype, weight, eps};
+  DropArg drop;
+  int rc = check_tokens(t);
+  if (rc == MG_OK) rc = check_norm(a);
+  if (rc == MG_OK) rc = drop_arg(p, seed, offset, state, &drop);
+  if (rc != MG_OK) return rc;
+  const size_t size = dtype_size(dtype), param_size = dtype_size(param_dtype);
+  if (!aligned(grad, size) || !aligned(table, size) || !aligned(grad_table, size) ||
+      !aligned(grad_weight, param_size) || !aligned(grad_bias, param_size))
+    return MG_ERR_INVALID_ARGUMENT;
+  const bool any = grad_table != nullptr || grad_weight != nullptr || grad_bias != nullptr;
+  if (channels == 0 || !any) return MG_OK;
+  if (nrows > 0) {
+    if (table == nullptr) return MG_ERR_NULL_POINTER;
+    if (ntokens > 0 && (type_index == nullptr || grad == nullptr)) return MG_ERR_NULL_POINTER;
+    rc = check_workspace(workspace, workspace_bytes,
+                         mg_encode_types_backward_workspace_size(ntokens, nrows, channels));
+    if (rc != MG_OK) return rc;
+  }
+  float* sums = static_cast<float*>(workspace);
+  const size_t sums_bytes = ((size_t)nrows * channels * sizeof(float) + 255) / 256 * 256;
+  void* rest = nrows > 0 ? static_cast<char*>(workspace) + sums_bytes : nullptr;
+  if (nrows > 0) {
+    rc = from_hip(launch_row_sums(t, grad, drop, sums, rest, workspace_bytes - sums_bytes,
+                                  (hipStream_t)stream));
+    if (rc != MG_OK) return rc;
+  }
+  return from_hip(launch_table_norm_backward(a, sums, table, scale, grad_table, grad_weight,
+                                             grad_bias, rest, (hipStream_t)stream));
+}
 
 }  // extern "C"

@@ -1,0 +1,139 @@
+// What the kernels of learned type vectors share: element types that are computed with in float,
+// several elements at a time, row numbers out of type indices, and the counter-based generator.
+#ifndef LIBMOLGRID_AMD_ELEMENT_TYPES_H_
+#define LIBMOLGRID_AMD_ELEMENT_TYPES_H_
+
+#include "device_common.h"
+
+namespace mg {
+
+// The tokens of a call: type indices and the table whose rows they name.
+struct TokenArg {
+  const void* index;  // ntokens indices of kind MG_INDEX_*
+  int ntokens, nrows, channels;
+  int dtype;  // MG_FLOAT32, ...: of the table and the type vectors
+  int index_kind;
+};
+
+// A layer norm: rows of `channels` elements.
+struct NormArg {
+  int nrows, channels;
+  int dtype, param_dtype;
+  const void* weight;  // channels elements, or nullptr for ones
+  float eps;
+};
+
+// Which elements a call drops.  Element e of the flattened array takes half e % 8 (low half of a
+// word first) of the words of counter (e / 8, offset) under key seed, and is kept where that half
+// is at least `limit`; `factor` multiplies what is kept.  16 bits an element: one counter serves
+// eight of them, so that the generator (about 500 cycles a wave and counter) stays behind the
+// memory it runs beside; with 32 bits an element it would be the bound for 16-bit types.
+struct DropArg {
+  uint32_t limit;         // round(65536 p): 0 keeps everything, 65536 nothing
+  float factor;           // 65536 / (65536 - limit), 0 when nothing is kept
+  uint64_t seed, offset;  // unless state is given
+  const uint64_t* state;  // device: {seed, offset}
+};
+// Arrays of 16-bit types are read and written as their bits; everything is computed in float and
+// rounded once, to the nearest, where it is stored.
+struct Half {
+  uint16_t bits;
+};
+struct Bfloat16 {
+  uint16_t bits;
+};
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(Half v) { return half_bits_to_float(v.bits); }
+__device__ __forceinline__ float widen(Bfloat16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
+
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ Half narrow<Half>(float v) {
+  return Half{float_to_half_bits(v)};
+}
+template <>
+__device__ __forceinline__ Bfloat16 narrow<Bfloat16>(float v) {
+  return Bfloat16{float_to_bfloat16_bits(v)};
+}
+
+// VEC elements that are loaded and stored by one instruction (or two, above 16 bytes)
+template <typename T, int VEC>
+struct __align__(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_floats(const T* p, float (&out)[VEC]) {
+  const Pack<T, VEC> pack = *reinterpret_cast<const Pack<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = widen(pack.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_floats(T* p, const float (&in)[VEC]) {
+  Pack<T, VEC> pack;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) pack.v[i] = narrow<T>(in[i]);
+  *reinterpret_cast<Pack<T, VEC>*>(p) = pack;
+}
+
+// Row of the table that a type index names, or -1 for one that names none.  A float index counts
+// as the whole number below it, as in the forward splat; not-a-number names no row.
+__device__ __forceinline__ int table_row(float index, int nrows) {
+  if (!(index >= 0.f && index < 2147483648.f)) return -1;
+  const int row = (int)index;
+  return row < nrows ? row : -1;
+}
+__device__ __forceinline__ int table_row(int32_t index, int nrows) {
+  return index >= 0 && index < nrows ? index : -1;
+}
+__device__ __forceinline__ int table_row(int64_t index, int nrows) {
+  return index >= 0 && index < (int64_t)nrows ? (int)index : -1;
+}
+
+// Sum over the lanes of a wave, in every lane.
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int m = kWave / 2; m > 0; m /= 2) v += __shfl_xor(v, m);
+  return v;
+}
+
+// Philox4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as
+// 1, 2, 3", SC 2011): four 32-bit words out of a 128-bit counter and a 64-bit key.
+struct Words4 {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Words4 philox(uint64_t low, uint64_t high, uint64_t key) {
+  uint32_t c0 = (uint32_t)low, c1 = (uint32_t)(low >> 32);
+  uint32_t c2 = (uint32_t)high, c3 = (uint32_t)(high >> 32);
+  uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+#pragma unroll
+  for (int round = 0; round < 10; ++round) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+    const uint32_t n0 = (uint32_t)(b >> 32) ^ c1 ^ k0, n2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)b;
+    c3 = (uint32_t)a;
+    c0 = n0;
+    c2 = n2;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return Words4{{c0, c1, c2, c3}};
+}
+
+__device__ __forceinline__ void drop_key(const DropArg& a, uint64_t& seed, uint64_t& offset) {
+  seed = a.state ? a.state[0] : a.seed;
+  offset = a.state ? a.state[1] : a.offset;
+}
+__device__ __forceinline__ uint32_t drop_half(const Words4& words, int i) {
+  return i & 1 ? words.w[i >> 1] >> 16 : words.w[i >> 1] & 0xFFFFu;
+}
+
+}  // namespace mg
+
+#endif

@@ -1,8 +1,9 @@
-// The inline assembly of the gfx950 kernels, in one place.
+// The inline assembly of the gfx950 kernels and their conversions of 16-bit types, in one place.
 #ifndef LIBMOLGRID_AMD_GFX950_ASM_H_
 #define LIBMOLGRID_AMD_GFX950_ASM_H_
 
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 namespace mg {
 
@@ -37,6 +38,17 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 // a wave's accesses, so the hardware needs no instruction here; this only keeps the compiler from
 // moving LDS accesses across the point.
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_wave_barrier(); }
+
+// Bits of a 16-bit float type from a float (to the nearest, ties to even) and back.
+__device__ __forceinline__ float half_bits_to_float(uint16_t bits) {
+  return (float)__builtin_bit_cast(_Float16, bits);
+}
+__device__ __forceinline__ uint16_t float_to_half_bits(float v) {
+  return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+__device__ __forceinline__ uint16_t float_to_bfloat16_bits(float v) {
+  return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
 
 }  // namespace mg
 

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include "device_common.h"
+#include "element_types.h"
 
 namespace mg {
 
@@ -114,6 +115,39 @@ hipError_t launch_interpolate(const InterpArg& p, int nbatch, const Vec3Arg& in_
                               const float* in, const Vec4Arg& quats, const Vec3Arg& rot_centers,
                               const Vec3Arg& translations, const Vec3Arg& out_centers, float* out,
                               hipStream_t stream);
+
+// Learned type vectors (embed.hip, layer_norm.hip, dropout.hip)
+hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const float* scales,
+                        void* out, hipStream_t stream);
+// The gradient of the table, and the sums of the kept, scaled-up gradients of every row's tokens
+// in float (the first half of launch_encode's backward pass); both need
+// row_sums_workspace_bytes().
+size_t row_sums_workspace_bytes(int ntokens, int nrows, int channels);
+hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scale,
+                                 const float* scales, void* grad_table, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+hipError_t launch_row_sums(const TokenArg& t, const void* grad, const DropArg& drop, float* out,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
+                                 float* grad_scales, hipStream_t stream);
+
+hipError_t launch_norm(const NormArg& a, const void* x, const void* bias, void* out, float* means,
+                       float* rstds, hipStream_t stream);
+size_t norm_backward_workspace_bytes(int nrows, int channels);
+hipError_t launch_norm_backward(const NormArg& a, const void* grad, const void* x,
+                                const float* means, const float* rstds, void* grad_x,
+                                void* grad_weight, void* grad_bias, void* workspace,
+                                hipStream_t stream);
+// The same for the rows of a scaled table and a float gradient; the statistics are computed again.
+hipError_t launch_table_norm_backward(const NormArg& a, const float* sums, const void* table,
+                                      float scale, void* grad_table, void* grad_weight,
+                                      void* grad_bias, void* workspace, hipStream_t stream);
+
+hipError_t launch_dropout(const void* in, size_t n, int dtype, const DropArg& drop, void* out,
+                          hipStream_t stream);
+
+hipError_t launch_encode(const TokenArg& t, const NormArg& a, const void* table, float scale,
+                         const void* bias, const DropArg& drop, void* out, hipStream_t stream);
 
 // float <-> double copies (convert.hip)
 hipError_t launch_widen(const float* src, double* dst, size_t n, hipStream_t stream);

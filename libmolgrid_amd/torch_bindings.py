@@ -87,14 +87,21 @@ class BatchedCoords2GridFunction(torch.autograd.Function):
 
 class Coords2Grid(torch.nn.Module):
     """Layer turning coordinates / type vectors / radii into a grid with a fixed GridMaker and
-    grid centre; accepts one example or a padded batch."""
+    grid centre; accepts one example or a padded batch.  With a ``type_encoder`` (TypeEncoder,
+    TypeEmbedding or another module from type indices to type vectors) the types may be type
+    indices, as MolMapDataset's items hold them: the grid's channels are the encoder's, and the
+    grid is differentiable in its parameters."""
 
-    def __init__(self, gmaker, center=(0, 0, 0)):
+    def __init__(self, gmaker, center=(0, 0, 0), type_encoder=None):
         super().__init__()
         self.gmaker = gmaker
         self.center = center
+        self.type_encoder = type_encoder
 
     def forward(self, coords, types, radii):
+        if self.type_encoder is not None and types.dim() == coords.dim() - 1:
+            # (the gridding kernels read float32 vectors whatever the encoder computes in)
+            types = self.type_encoder(types).float()
         coords, types, radii = coords.contiguous(), types.contiguous(), radii.contiguous()
         if coords.dim() == 3 and types.dim() == 3 and radii.dim() == 2:
             return BatchedCoords2GridFunction.apply(self.gmaker, self.center, coords, types, radii)

@@ -9,7 +9,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 CSRC = os.path.join(ROOT, "libmolgrid_amd", "csrc")
 SOURCES = ["capi.hip", "transform.hip", "convert.hip", "forward_sorted.hip", "forward_vector.hip",
-           "forward_vector_mfma.hip", "backward.hip", "second_order.hip", "interpolate.hip"]
+           "forward_vector_mfma.hip", "backward.hip", "second_order.hip", "interpolate.hip",
+           "embed.hip", "layer_norm.hip", "dropout.hip"]
 
 # EMU_SANITIZE selects a second build of the same sources with clang's run-time checks, every report
 # fatal: "1" the undefined-behaviour checks (array indices of fixed-size arrays -- the register and

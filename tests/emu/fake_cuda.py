@@ -143,6 +143,7 @@ def activate():
     torch.cuda.set_device = lambda d: None
     torch.cuda.current_device = lambda: 0
     torch.cuda.synchronize = lambda *a, **k: None
+    torch.cuda.is_current_stream_capturing = lambda: False
     torch.cuda.current_stream = lambda *a, **k: FakeStream()
     torch.cuda.Stream = FakeStream
     torch.cuda.Event = FakeEvent
@@ -176,3 +177,11 @@ def activate():
         return real_to(self, *a, **k)
     torch.Tensor.to = to
     torch.Tensor.record_stream = lambda self, s: None
+
+    def module_cuda(self, *a, **k):
+        for m in self.modules():
+            for name, value in m._parameters.items():
+                if value is not None:
+                    m._parameters[name] = torch.nn.Parameter(on_device(value.data.clone()))
+        return self
+    torch.nn.Module.cuda = module_cuda

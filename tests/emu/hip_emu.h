@@ -288,4 +288,26 @@ inline void compute_here(int&) {}
 inline void lds_barrier() { emu::barrier(); }
 // the lanes of a wave are fibers here and do not run in step: meet
 inline void wave_lds_fence() { uint64_t live; (void)emu::gather(0, &live, "wave_lds_fence"); }
+// conversions of the 16-bit types, to the nearest with ties to even
+inline float half_bits_to_float(uint16_t h) {
+  const int e = (h >> 10) & 31, m = h & 1023;
+  const float v = e == 31 ? (m ? NAN : INFINITY) : e ? ldexpf((float)(1024 + m), e - 25) : ldexpf((float)m, -24);
+  return h >> 15 ? -v : v;
+}
+inline uint16_t float_to_half_bits(float f) {
+  const uint32_t u = __float_as_uint(f);
+  const uint16_t sign = (uint16_t)((u >> 16) & 0x8000u);
+  if (f != f) return sign | 0x7E00u;
+  const float a = fabsf(f);
+  if (a >= 65520.f) return sign | 0x7C00u;
+  if (a < 6.103515625e-5f) return sign | (uint16_t)nearbyintf(ldexpf(a, 24));   // subnormal steps of 2^-24
+  int e;
+  const float m = frexpf(a, &e);                                                 // [0.5, 1) * 2^e
+  return sign | (uint16_t)(((uint32_t)(e + 14) << 10) + (uint32_t)nearbyintf(ldexpf(m, 11)) - 1024u);
+}
+inline uint16_t float_to_bfloat16_bits(float f) {
+  const uint32_t u = __float_as_uint(f);
+  if (f != f) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
 }  // namespace mg
