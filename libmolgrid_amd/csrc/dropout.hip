@@ -2,37 +2,62 @@
 // so the backward pass is the same call on the gradient.
 #include "element_types.h"
 #include "kernels.h"
+#include "row_team.h"
 
 namespace mg {
 namespace {
 
 constexpr int kThreads = 256;
 
-// One thread takes one group of eight elements, i.e. one counter of the generator.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void dropout_kernel(const T* in, size_t n, DropArg drop,
+// A thread takes kGroups groups of eight elements, i.e. as many counters of the generator, and has
+// their loads in flight together.  WHOLE: the arrays start on 16-byte boundaries.
+constexpr int kGroups = 2;
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void dropout_kernel(const T* in, size_t n, DropArg arg,
                                                            T* out) {
   uint64_t seed, offset;
-  drop_key(drop, seed, offset);
-  const size_t groups = (n + 7) / 8, stride = (size_t)gridDim.x * kThreads;
-  for (size_t g = (size_t)blockIdx.x * kThreads + threadIdx.x; g < groups; g += stride) {
-    const Words4 words = philox(g, offset, seed);
+  drop_key(arg, seed, offset);
+  const size_t groups = (n + 7) / 8;
+  for (size_t g0 = (size_t)blockIdx.x * kThreads * kGroups + threadIdx.x; g0 < groups;
+       g0 += (size_t)gridDim.x * kThreads * kGroups) {
+    float v[kGroups][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const size_t e = g * 8 + i;
-      if (e >= n) break;
-      const float v = widen(in[e]) * drop.factor;
-      out[e] = narrow<T>(drop_half(words, i) >= drop.limit ? v : 0.f);
+    for (int j = 0; j < kGroups; ++j) {
+      const size_t e = (g0 + (size_t)j * kThreads) * 8;
+      if (WHOLE && e + 8 <= n) {
+        load_floats<T, 8>(in + e, v[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = e + i < n ? widen(in[e + i]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      const size_t e = (g0 + (size_t)j * kThreads) * 8;
+      drop<8>(e, arg, seed, offset, v[j]);
+      if (WHOLE && e + 8 <= n) {
+        store_floats<T, 8>(out + e, v[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (e + i < n) out[e + i] = narrow<T>(v[j][i]);
+      }
     }
   }
 }
 
 template <typename T>
-hipError_t dropout(const void* in, size_t n, const DropArg& drop, void* out, hipStream_t stream) {
-  size_t blocks = ((n + 7) / 8 + kThreads - 1) / kThreads;
-  if (blocks > 65536) blocks = 65536;
-  hipLaunchKernelGGL((dropout_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
-                     (const T*)in, n, drop, (T*)out);
+hipError_t dropout(const void* in, size_t n, const DropArg& arg, void* out, hipStream_t stream) {
+  const size_t share = (size_t)kThreads * kGroups * 8;
+  size_t blocks = (n + share - 1) / share;
+  if (blocks > 1u << 20) blocks = 1u << 20;
+  if ((address(in) | address(out)) % 16 == 0)
+    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                       (const T*)in, n, arg, (T*)out);
+  else
+    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                       (const T*)in, n, arg, (T*)out);
   return hipGetLastError();
 }
 

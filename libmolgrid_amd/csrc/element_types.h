@@ -96,6 +96,14 @@ __device__ __forceinline__ int table_row(int64_t index, int nrows) {
   return index >= 0 && index < (int64_t)nrows ? (int)index : -1;
 }
 
+__device__ __forceinline__ int token_row(const TokenArg& t, size_t n) {
+  switch (t.index_kind) {   // (the same in every lane)
+    case MG_INDEX_FLOAT32: return table_row(static_cast<const float*>(t.index)[n], t.nrows);
+    case MG_INDEX_INT32: return table_row(static_cast<const int32_t*>(t.index)[n], t.nrows);
+    default: return table_row(static_cast<const int64_t*>(t.index)[n], t.nrows);
+  }
+}
+
 // Sum over the lanes of a wave, in every lane.
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll

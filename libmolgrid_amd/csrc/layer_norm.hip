@@ -6,8 +6,10 @@
 //
 // The variance is that of the differences, not mean x^2 - m^2, which loses its digits where |m| is
 // large beside the spread.  Statistics and sums are float throughout.
-#include "element_types.h"
+#include <type_traits>
+
 #include "kernels.h"
+#include "row_team.h"
 
 namespace mg {
 namespace {
@@ -20,219 +22,475 @@ struct Stats {
 };
 
 template <typename T>
-__device__ __forceinline__ Stats row_stats(const T* x, int channels, float scale, float eps,
-                                           int lane) {
-  float sum = 0.f;
-  for (int c = lane; c < channels; c += kWave) sum += scale * widen(x[c]);
-  const float mean = lanes_sum(sum) / channels;
-  float squares = 0.f;
-  for (int c = lane; c < channels; c += kWave) {
-    const float d = scale * widen(x[c]) - mean;
-    squares = fmaf(d, d, squares);
-  }
-  return Stats{mean, 1.f / sqrtf(lanes_sum(squares) / channels + eps)};
+__device__ __forceinline__ float param_at(const void* p, bool is_float, int c, float absent) {
+  if (p == nullptr) return absent;
+  return is_float ? static_cast<const float*>(p)[c] : widen(static_cast<const T*>(p)[c]);
 }
 
-// A wave takes one row.
-template <typename T, typename P>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const T* x, int nrows, int channels,
-                                                        const P* __restrict__ weight,
-                                                        const P* __restrict__ bias, float eps,
-                                                        T* out, float* __restrict__ means,
-                                                        float* __restrict__ rstds) {
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int n = blockIdx.x * kWaves + threadIdx.x / kWave; n < nrows; n += gridDim.x * kWaves) {
-    const T* row = x + (size_t)n * channels;
-    const Stats s = row_stats(row, channels, 1.f, eps, lane);
-    for (int c = lane; c < channels; c += kWave) {
-      const float h = (widen(row[c]) - s.mean) * s.rstd;
-      out[(size_t)n * channels + c] =
-          narrow<T>(fmaf(h, weight ? widen(weight[c]) : 1.f, bias ? widen(bias[c]) : 0.f));
+// Statistics of one row by the whole workgroup.
+template <typename T>
+__device__ __forceinline__ Stats wide_row_stats(const T* x, int channels, float scale, float eps,
+                                                float (&slots)[2][kWaves]) {
+  float sum[1] = {0.f}, squares[1] = {0.f};
+  for (int c = threadIdx.x; c < channels; c += kThreads) sum[0] += scale * widen(x[c]);
+  team_sums<kThreads>(sum, slots[0]);
+  const float mean = sum[0] / channels;
+  for (int c = threadIdx.x; c < channels; c += kThreads) {
+    const float d = scale * widen(x[c]) - mean;
+    squares[0] = fmaf(d, d, squares[0]);
+  }
+  team_sums<kThreads>(squares, slots[1]);
+  return Stats{mean, 1.f / sqrtf(squares[0] / channels + eps)};
+}
+
+// Forward: a team holds a row in registers, sums it and its squared differences and writes it once.
+// The workgroups stay (kResident of them) and go through the rows, so that a lane reads its share of
+// weight and bias once; the next row's loads are in flight while a row is summed.
+// ENCODE: the rows are those of a scaled table, by the tokens' indices, and are dropped out.
+constexpr int kResident = 2048;
+
+template <typename T, int VEC, int LANES, int K, bool ENCODE>
+__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
+    const T* x, TokenArg tokens, float scale, NormArg a, const void* __restrict__ bias, DropArg arg,
+    T* out, float* __restrict__ means, float* __restrict__ rstds) {
+  using Shape = TeamShape<LANES, K>;
+  __shared__ float slots[2][Shape::WAVES];
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  const int channels = a.channels;
+  const uint32_t nrows = (uint32_t)(ENCODE ? tokens.ntokens : a.nrows);
+  uint64_t seed = 0, offset = 0;
+  if (ENCODE) drop_key(arg, seed, offset);
+  float w[K][VEC], b[K][VEC];
+  load_param<T, VEC, LANES, K>(a.weight, a.param_dtype == MG_FLOAT32, 1.f, channels, lane, w);
+  load_param<T, VEC, LANES, K>(bias, a.param_dtype == MG_FLOAT32, 0.f, channels, lane, b);
+  const float inv = 1.f / channels;
+  const uint32_t step = gridDim.x * Shape::TEAMS;
+
+  RowPacks<T, VEC, K> next;
+  bool next_named = true;
+  const auto fetch = [&](uint32_t n) {
+    size_t at = n;
+    bool live = n < nrows;
+    if (ENCODE) {
+      const int row = live ? token_row(tokens, n) : -1;
+      at = row < 0 ? 0 : row;
+      live = next_named = row >= 0;
     }
-    if (lane == 0 && means) {
+    load_row<T, VEC, LANES, K>(x + at * channels, channels, lane, live, next);
+  };
+  fetch(blockIdx.x * Shape::TEAMS + team);
+  for (uint32_t n0 = blockIdx.x * Shape::TEAMS; n0 < nrows; n0 += step) {
+    const uint32_t n = n0 + team;
+    const RowPacks<T, VEC, K> packs = next;
+    const bool named = next_named;
+    fetch(n + step);
+    float v[K][VEC];
+    float sum[1] = {0.f}, squares[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[k][i] = widen(packs.pack[k].v[i]);
+        if (ENCODE) v[k][i] *= scale;
+        sum[0] += v[k][i];
+      }
+    team_sums<LANES>(sum, slots[0]);
+    const float mean = sum[0] / channels;   // (a product could be contracted into the differences)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool inside = (k * LANES + lane) * VEC < channels;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[k][i] = inside ? v[k][i] - mean : 0.f;
+        squares[0] = fmaf(v[k][i], v[k][i], squares[0]);
+      }
+    }
+    team_sums<LANES>(squares, slots[1]);
+    const float rstd = 1.f / sqrtf(fmaf(squares[0], inv, a.eps));
+    if (n >= nrows) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c >= channels) break;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[k][i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
+      const size_t e = (size_t)n * channels + c;
+      if (ENCODE) {
+        drop<VEC>(e, arg, seed, offset, v[k]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[k][i] = named ? v[k][i] : 0.f;
+      }
+      store_floats<T, VEC>(out + e, v[k]);
+    }
+    if (!ENCODE && means && lane == 0) {
+      means[n] = mean;
+      rstds[n] = rstd;
+    }
+  }
+}
+
+// Rows wider than any team (more than 16,384 channels): a workgroup goes over the row three times,
+// which stays in the caches.
+template <typename T, bool ENCODE>
+__global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenArg tokens,
+                                                             float scale, NormArg a,
+                                                             const void* __restrict__ bias,
+                                                             DropArg arg, T* out,
+                                                             float* __restrict__ means,
+                                                             float* __restrict__ rstds) {
+  __shared__ float slots[2][kWaves];
+  uint64_t seed = 0, offset = 0;
+  if (ENCODE) drop_key(arg, seed, offset);
+  const bool is_float = a.param_dtype == MG_FLOAT32;
+  const uint32_t nrows = (uint32_t)(ENCODE ? tokens.ntokens : a.nrows);
+  for (uint32_t n = blockIdx.x; n < nrows; n += gridDim.x) {
+    const int at = ENCODE ? token_row(tokens, n) : 0;
+    T* to = out + (size_t)n * a.channels;
+    if (at < 0) {
+      for (int c = threadIdx.x; c < a.channels; c += kThreads) to[c] = narrow<T>(0.f);
+      continue;
+    }
+    const T* row = x + (size_t)(ENCODE ? (uint32_t)at : n) * a.channels;
+    const Stats s = wide_row_stats(row, a.channels, ENCODE ? scale : 1.f, a.eps, slots);
+    for (int c = threadIdx.x; c < a.channels; c += kThreads) {
+      const float h = ((ENCODE ? scale : 1.f) * widen(row[c]) - s.mean) * s.rstd;
+      float y[1] = {fmaf(h, param_at<T>(a.weight, is_float, c, 1.f), param_at<T>(bias, is_float, c, 0.f))};
+      if (ENCODE) drop<1>((size_t)n * a.channels + c, arg, seed, offset, y);
+      to[c] = narrow<T>(y[0]);
+    }
+    if (!ENCODE && means && threadIdx.x == 0) {
       means[n] = s.mean;
       rstds[n] = s.rstd;
     }
   }
 }
 
-template <typename T, typename P, typename I>
-__global__ __launch_bounds__(kThreads) void encode_kernel(const I* __restrict__ index,
-                                                          const T* __restrict__ table, int ntokens,
-                                                          int nrows, int channels, float scale,
-                                                          const P* __restrict__ weight,
-                                                          const P* __restrict__ bias, float eps,
-                                                          DropArg drop, T* __restrict__ out) {
-  uint64_t seed, offset;
-  drop_key(drop, seed, offset);
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int n = blockIdx.x * kWaves + threadIdx.x / kWave; n < ntokens; n += gridDim.x * kWaves) {
-    const int at = table_row(index[n], nrows);
-    if (at < 0) {
-      for (int c = lane; c < channels; c += kWave)
-        out[(size_t)n * channels + c] = narrow<T>(0.f);
-      continue;
-    }
-    const T* row = table + (size_t)at * channels;
-    const Stats s = row_stats(row, channels, scale, eps, lane);
-    for (int c = lane; c < channels; c += kWave) {
-      const float h = (scale * widen(row[c]) - s.mean) * s.rstd;
-      const float y = fmaf(h, weight ? widen(weight[c]) : 1.f, bias ? widen(bias[c]) : 0.f);
-      const size_t e = (size_t)n * channels + c;
-      const Words4 words = philox(e >> 3, offset, seed);
-      out[e] = narrow<T>(drop_half(words, (int)(e & 7)) >= drop.limit ? y * drop.factor : 0.f);
-    }
-  }
-}
+// Backward: a team holds the rows of x and of the gradient, writes dx, and a lane adds its share of
+// dw and db up over all rows that its team takes.  At the end the workgroup's teams are added in
+// their order, and the workgroup writes one row of `partial` (dw, then db).  G: type of the
+// gradient; TABLE: x is a scaled table, whose statistics are computed here.
+constexpr int kParts = 512;
 
-// dx; a wave takes one row.  G is float where the gradient is a sum over tokens.
-template <typename T, typename P, typename G>
-__global__ __launch_bounds__(kThreads) void norm_backward_kernel(
-    const G* grad, const T* x, int nrows, int channels, float scale, const float* means,
-    const float* rstds, const P* __restrict__ weight, float eps, T* grad_x) {
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int n = blockIdx.x * kWaves + threadIdx.x / kWave; n < nrows; n += gridDim.x * kWaves) {
-    const size_t at = (size_t)n * channels;
-    const Stats s = means ? Stats{means[n], rstds[n]} : row_stats(x + at, channels, scale, eps, lane);
-    float sum = 0.f, sum_h = 0.f;
-    for (int c = lane; c < channels; c += kWave) {
-      const float q = widen(grad[at + c]) * (weight ? widen(weight[c]) : 1.f);
-      sum += q;
-      sum_h = fmaf(q, (scale * widen(x[at + c]) - s.mean) * s.rstd, sum_h);
-    }
-    sum = lanes_sum(sum) / channels;
-    sum_h = lanes_sum(sum_h) / channels;
-    for (int c = lane; c < channels; c += kWave) {
-      const float q = widen(grad[at + c]) * (weight ? widen(weight[c]) : 1.f);
-      const float h = (scale * widen(x[at + c]) - s.mean) * s.rstd;
-      grad_x[at + c] = narrow<T>(scale * s.rstd * (q - sum - h * sum_h));
-    }
-  }
-}
+template <typename T, typename G, int VEC, int LANES, int K, bool TABLE>
+__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_kernel(
+    const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a,
+    const float* __restrict__ means, const float* __restrict__ rstds, T* __restrict__ grad_x,
+    float* __restrict__ partial) {
+  using Shape = TeamShape<LANES, K>;
+  __shared__ float slots[4][2 * Shape::WAVES];
+  HIP_DYNAMIC_SHARED(float, sums);   // dw and db of a workgroup with several teams
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  const int channels = a.channels;
+  const uint32_t nrows = (uint32_t)a.nrows;
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+  load_param<T, VEC, LANES, K>(a.weight, a.param_dtype == MG_FLOAT32, 1.f, channels, lane, w);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.f;
+  const float inv = 1.f / channels;
+  const uint32_t step = gridDim.x * Shape::TEAMS;
 
-// dw and db, first step: the workgroup's share of the rows is summed into its own row of `partial`
-// (weight, then bias).
-template <typename T, typename G>
-__global__ __launch_bounds__(kThreads) void norm_params_kernel(const G* grad, const T* x, int nrows,
-                                                               int channels, float scale,
-                                                               const float* means,
-                                                               const float* rstds, float eps,
-                                                               float* __restrict__ partial) {
-  __shared__ Stats stats[kThreads];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  for (int c0 = 0; c0 < channels; c0 += kThreads) {
-    const int c = c0 + threadIdx.x;
-    float dw = 0.f, db = 0.f;
-    for (int n0 = blockIdx.x * kThreads; n0 < nrows; n0 += gridDim.x * kThreads) {
-      const int count = min(kThreads, nrows - n0);
-      __syncthreads();
-      if (means) {
-        if ((int)threadIdx.x < count) stats[threadIdx.x] = Stats{means[n0 + threadIdx.x], rstds[n0 + threadIdx.x]};
-      } else {
-        for (int i = wave; i < count; i += kWaves)
-          stats[i] = row_stats(x + (size_t)(n0 + i) * channels, channels, scale, eps, lane);
-      }
-      __syncthreads();
-      if (c < channels)
-        for (int i = 0; i < count; ++i) {
-          const size_t at = (size_t)(n0 + i) * channels + c;
-          const float g = widen(grad[at]);
-          dw = fmaf(g, (scale * widen(x[at]) - stats[i].mean) * stats[i].rstd, dw);
-          db += g;
+  RowPacks<T, VEC, K> next_x;
+  RowPacks<G, VEC, K> next_g;
+  float next_mean = 0.f, next_rstd = 0.f;
+  const auto fetch = [&](uint32_t n) {
+    const bool live = n < nrows;
+    const size_t at = live ? (size_t)n * channels : 0;
+    load_row<T, VEC, LANES, K>(x + at, channels, lane, live, next_x);
+    load_row<G, VEC, LANES, K>(grad + at, channels, lane, live, next_g);
+    if (!TABLE && live) {
+      next_mean = means[n];
+      next_rstd = rstds[n];
+    }
+  };
+  fetch(blockIdx.x * Shape::TEAMS + team);
+  int parity = 0;   // a row's sums must not meet those of the row before in the same slots
+  for (uint32_t n0 = blockIdx.x * Shape::TEAMS; n0 < nrows; n0 += step, parity ^= 1) {
+    const uint32_t n = n0 + team;
+    const RowPacks<T, VEC, K> px = next_x;
+    const RowPacks<G, VEC, K> pg = next_g;
+    float mean = next_mean, rstd = next_rstd;
+    fetch(n + step);
+    float h[K][VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[k][i] = TABLE ? scale * widen(px.pack[k].v[i]) : widen(px.pack[k].v[i]);
+    if (TABLE) {
+      float sum[1] = {0.f}, squares[1] = {0.f};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[0] += h[k][i];
+      team_sums<LANES>(sum, slots[2]);
+      mean = sum[0] / channels;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float d = (k * LANES + lane) * VEC < channels ? h[k][i] - mean : 0.f;
+          squares[0] = fmaf(d, d, squares[0]);
         }
+      team_sums<LANES>(squares, slots[3]);
+      rstd = 1.f / sqrtf(fmaf(squares[0], inv, a.eps));
     }
-    if (c < channels) {
-      partial[(size_t)blockIdx.x * 2 * channels + c] = dw;
-      partial[((size_t)blockIdx.x * 2 + 1) * channels + c] = db;
+    float both[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float g = widen(pg.pack[k].v[i]);
+        h[k][i] = (h[k][i] - mean) * rstd;
+        const float q = g * w[k][i];
+        both[0] += q;
+        both[1] = fmaf(q, h[k][i], both[1]);
+        if (n < nrows) dw[k][i] = fmaf(g, h[k][i], dw[k][i]);
+        db[k][i] += g;
+      }
+    team_sums<LANES>(both, slots[parity]);
+    if (grad_x == nullptr || n >= nrows) continue;
+    const float mean_q = both[0] * inv, mean_qh = both[1] * inv;
+    const float factor = TABLE ? scale * rstd : rstd;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c >= channels) break;
+      float d[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float q = widen(pg.pack[k].v[i]) * w[k][i];
+        d[i] = factor * (q - mean_q - h[k][i] * mean_qh);
+      }
+      store_floats<T, VEC>(grad_x + (size_t)n * channels + c, d);
+    }
+  }
+  if (partial == nullptr) return;
+
+  // the teams of a wave, then the waves of the workgroup
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+      for (int m = LANES; m < kWave; m *= 2) {
+        dw[k][i] += __shfl_xor(dw[k][i], m);
+        db[k][i] += __shfl_xor(db[k][i], m);
+      }
+    }
+  constexpr int kTurns = LANES < kWave ? Shape::WAVES : Shape::TEAMS;   // one after the other
+  const int turn = LANES < kWave ? threadIdx.x / kWave : team;
+  const bool speaks = LANES >= kWave || (threadIdx.x & (kWave - 1)) < LANES;
+  for (int t = 0; t < kTurns; ++t) {
+    if (t > 0) lds_barrier();
+    if (turn != t || !speaks) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c >= channels) break;
+      float* to_w = partial + (size_t)blockIdx.x * 2 * channels + c;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (t > 0) {
+          dw[k][i] += sums[c + i];
+          db[k][i] += sums[channels + c + i];
+        }
+        if (t + 1 < kTurns) {
+          sums[c + i] = dw[k][i];
+          sums[channels + c + i] = db[k][i];
+        } else {
+          to_w[i] = dw[k][i];
+          to_w[channels + i] = db[k][i];
+        }
+      }
     }
   }
 }
 
-// Second step: the partial rows are summed in their order.
+// The same for rows wider than any team: dx, a workgroup a row, and dw and db, a thread a channel.
+template <typename T, typename G>
+__global__ __launch_bounds__(kThreads) void wide_norm_backward_kernel(
+    const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a, const float* means,
+    const float* rstds, T* __restrict__ grad_x) {
+  __shared__ float slots[2][kWaves];
+  __shared__ float both_slots[2 * kWaves];
+  const bool is_float = a.param_dtype == MG_FLOAT32;
+  for (int n = blockIdx.x; n < a.nrows; n += gridDim.x) {
+    const size_t at = (size_t)n * a.channels;
+    const Stats s = means ? Stats{means[n], rstds[n]}
+                          : wide_row_stats(x + at, a.channels, scale, a.eps, slots);
+    float both[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < a.channels; c += kThreads) {
+      const float q = widen(grad[at + c]) * param_at<T>(a.weight, is_float, c, 1.f);
+      both[0] += q;
+      both[1] = fmaf(q, (scale * widen(x[at + c]) - s.mean) * s.rstd, both[1]);
+    }
+    lds_barrier();
+    team_sums<kThreads>(both, both_slots);
+    const float mean_q = both[0] / a.channels, mean_qh = both[1] / a.channels;
+    for (int c = threadIdx.x; c < a.channels; c += kThreads) {
+      const float q = widen(grad[at + c]) * param_at<T>(a.weight, is_float, c, 1.f);
+      const float h = (scale * widen(x[at + c]) - s.mean) * s.rstd;
+      grad_x[at + c] = narrow<T>(scale * s.rstd * (q - mean_q - h * mean_qh));
+    }
+  }
+}
+
+template <typename T, typename G>
+__global__ __launch_bounds__(kThreads) void wide_norm_params_kernel(
+    const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a, const float* means,
+    const float* rstds, float* __restrict__ partial) {
+  __shared__ float slots[2][kWaves];
+  float* row = partial + (size_t)blockIdx.x * 2 * a.channels;
+  for (int c = threadIdx.x; c < a.channels; c += kThreads) row[c] = row[a.channels + c] = 0.f;
+  for (int n = blockIdx.x; n < a.nrows; n += gridDim.x) {
+    const size_t at = (size_t)n * a.channels;
+    const Stats s = means ? Stats{means[n], rstds[n]}
+                          : wide_row_stats(x + at, a.channels, scale, a.eps, slots);
+    for (int c = threadIdx.x; c < a.channels; c += kThreads) {   // (the same thread all along)
+      const float g = widen(grad[at + c]);
+      row[c] = fmaf(g, (scale * widen(x[at + c]) - s.mean) * s.rstd, row[c]);
+      row[a.channels + c] += g;
+    }
+  }
+}
+
+// The rows of `partial`, summed: a workgroup takes 64 columns (of dw, then db), its waves a share
+// of the rows each, which are then added in their order.
+constexpr int kSumWaves = 16;
+
 template <typename P>
-__global__ __launch_bounds__(kThreads) void norm_params_sum_kernel(const float* __restrict__ partial,
-                                                                   int parts, int channels,
-                                                                   P* __restrict__ grad_weight,
-                                                                   P* __restrict__ grad_bias) {
-  for (int c = blockIdx.x * kThreads + threadIdx.x; c < channels; c += gridDim.x * kThreads) {
-    float dw = 0.f, db = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      dw += partial[(size_t)i * 2 * channels + c];
-      db += partial[((size_t)i * 2 + 1) * channels + c];
-    }
-    if (grad_weight) grad_weight[c] = narrow<P>(dw);
-    if (grad_bias) grad_bias[c] = narrow<P>(db);
-  }
+__global__ __launch_bounds__(kWave* kSumWaves) void sum_partials_kernel(
+    const float* __restrict__ partial, int parts, int channels, P* __restrict__ grad_weight,
+    P* __restrict__ grad_bias) {
+  __shared__ float sums[kSumWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const size_t columns = (size_t)2 * channels, c = (size_t)blockIdx.x * kWave + lane;
+  const int share = (parts + kSumWaves - 1) / kSumWaves;
+  const int end = min(parts, (wave + 1) * share);
+  float sum = 0.f;
+  if (c < columns)
+#pragma unroll 8
+    for (int i = wave * share; i < end; ++i) sum += partial[(size_t)i * columns + c];
+  sums[wave][lane] = sum;
+  lds_barrier();
+  if (wave != 0 || c >= columns) return;
+  for (int w = 1; w < kSumWaves; ++w) sum += sums[w][lane];
+  P* to = c < (size_t)channels ? grad_weight : grad_bias;
+  if (to) to[c < (size_t)channels ? c : c - channels] = narrow<P>(sum);
 }
 
-unsigned row_blocks(int nrows) {
-  const size_t blocks = ((size_t)nrows + kWaves - 1) / kWaves;
-  return (unsigned)(blocks < 65536 ? (blocks ? blocks : 1) : 65536);
-}
-int norm_parts(int nrows) { return nrows >= 512 * 256 ? 512 : (nrows + 255) / 256; }
+int wide_parts(int nrows) { return nrows < 256 ? nrows : 256; }
 
-template <typename T, typename P>
-hipError_t norm(const NormArg& a, const void* x, const void* bias, void* out, float* means,
-                float* rstds, hipStream_t stream) {
-  hipLaunchKernelGGL((norm_kernel<T, P>), dim3(row_blocks(a.nrows)), dim3(kThreads), 0, stream,
-                     (const T*)x, a.nrows, a.channels, (const P*)a.weight, (const P*)bias, a.eps,
-                     (T*)out, means, rstds);
+template <typename P>
+void sum_partials(const float* partial, int parts, int channels, void* grad_weight, void* grad_bias,
+                  hipStream_t stream) {
+  hipLaunchKernelGGL((sum_partials_kernel<P>), dim3(((size_t)2 * channels + kWave - 1) / kWave),
+                     dim3(kWave * kSumWaves), 0, stream, partial, parts, channels, (P*)grad_weight,
+                     (P*)grad_bias);
+}
+
+template <typename T, bool ENCODE>
+hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x, const void* bias,
+                const DropArg& drop, void* out, float* means, float* rstds, hipStream_t stream) {
+  const uint32_t nrows = (uint32_t)(ENCODE ? t.ntokens : a.nrows);
+  const auto with_packs = [&](auto vec) {
+    constexpr int VEC = decltype(vec)::value;
+    return with_team<VEC>((a.channels + VEC - 1) / VEC, [&](auto shape) {
+      using S = decltype(shape);
+      const uint32_t blocks = (nrows + S::TEAMS - 1) / S::TEAMS;
+      const uint32_t resident = kResident * 256 / S::THREADS;
+      hipLaunchKernelGGL((norm_kernel<T, VEC, S::LANES, S::K, ENCODE>),
+                         dim3(blocks < resident ? blocks : resident), dim3(S::THREADS), 0, stream,
+                         (const T*)x, t, scale, a, bias, drop, (T*)out, means, rstds);
+    });
+  };
+  const bool done = whole_packs<T>(a.channels, address(x) | address(out))
+                        ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
+                        : with_packs(std::integral_constant<int, 1>());
+  if (!done)
+    hipLaunchKernelGGL((wide_norm_kernel<T, ENCODE>), dim3(nrows < 4096 ? nrows : 4096),
+                       dim3(kThreads), 0, stream, (const T*)x, t, scale, a, bias, drop, (T*)out,
+                       means, rstds);
   return hipGetLastError();
 }
 
-template <typename T, typename P, typename G>
+// Workgroups that share the rows, each with its row of partial sums: as many as fill the chip, but
+// no more than rows for eight rounds where the sums' own traffic (8 bytes a channel and workgroup)
+// would not be small beside that of the rows.
+int norm_parts(int nrows, int teams) {
+  const size_t rounds = ((size_t)nrows + teams - 1) / teams;
+  return (int)(rounds < kParts ? rounds : kParts);
+}
+
+template <typename T, typename G, bool TABLE>
 hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, float scale,
                          const float* means, const float* rstds, void* grad_x, void* grad_weight,
                          void* grad_bias, void* workspace, hipStream_t stream) {
-  if (grad_x && a.nrows > 0)
-    hipLaunchKernelGGL((norm_backward_kernel<T, P, G>), dim3(row_blocks(a.nrows)), dim3(kThreads), 0,
-                       stream, (const G*)grad, (const T*)x, a.nrows, a.channels, scale, means, rstds,
-                       (const P*)a.weight, a.eps, (T*)grad_x);
-  if (grad_weight || grad_bias) {
-    const int parts = norm_parts(a.nrows);
-    if (parts > 0)
-      hipLaunchKernelGGL((norm_params_kernel<T, G>), dim3(parts), dim3(kThreads), 0, stream,
-                         (const G*)grad, (const T*)x, a.nrows, a.channels, scale, means, rstds, a.eps,
-                         (float*)workspace);
-    hipLaunchKernelGGL((norm_params_sum_kernel<P>), dim3((a.channels + kThreads - 1) / kThreads),
-                       dim3(kThreads), 0, stream, (const float*)workspace, parts, a.channels,
-                       (P*)grad_weight, (P*)grad_bias);
+  const bool to_params = grad_weight || grad_bias;
+  float* partial = to_params ? static_cast<float*>(workspace) : nullptr;
+  int parts = 0;
+  if (a.nrows > 0) {
+    const auto with_packs = [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      return with_team<VEC>((a.channels + VEC - 1) / VEC, [&](auto shape) {
+        using S = decltype(shape);
+        parts = norm_parts(a.nrows, S::TEAMS);
+        const size_t shared = S::LANES <= kWave ? (size_t)2 * a.channels * sizeof(float) : 0;
+        hipLaunchKernelGGL((norm_backward_kernel<T, G, VEC, S::LANES, S::K, TABLE>), dim3(parts),
+                           dim3(S::THREADS), shared, stream, (const G*)grad, (const T*)x, scale, a,
+                           means, rstds, (T*)grad_x, partial);
+      });
+    };
+    const bool whole = whole_packs<T>(a.channels, address(x) | address(grad) | address(grad_x));
+    const bool done = whole ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
+                            : with_packs(std::integral_constant<int, 1>());
+    if (!done) {
+      parts = wide_parts(a.nrows);
+      if (grad_x)
+        hipLaunchKernelGGL((wide_norm_backward_kernel<T, G>), dim3(a.nrows < 4096 ? a.nrows : 4096),
+                           dim3(kThreads), 0, stream, (const G*)grad, (const T*)x, scale, a, means,
+                           rstds, (T*)grad_x);
+      if (partial)
+        hipLaunchKernelGGL((wide_norm_params_kernel<T, G>), dim3(parts), dim3(kThreads), 0, stream,
+                           (const G*)grad, (const T*)x, scale, a, means, rstds, partial);
+    }
   }
-  return hipGetLastError();
-}
-
-template <typename T, typename P, typename I>
-hipError_t encode(const TokenArg& t, const NormArg& a, const void* table, float scale,
-                  const void* bias, const DropArg& drop, void* out, hipStream_t stream) {
-  hipLaunchKernelGGL((encode_kernel<T, P, I>), dim3(row_blocks(t.ntokens)), dim3(kThreads), 0,
-                     stream, (const I*)t.index, (const T*)table, t.ntokens, t.nrows, t.channels,
-                     scale, (const P*)a.weight, (const P*)bias, a.eps, drop, (T*)out);
+  if (to_params) {
+    if (a.param_dtype == MG_FLOAT32)
+      sum_partials<float>(partial, parts, a.channels, grad_weight, grad_bias, stream);
+    else
+      sum_partials<T>(partial, parts, a.channels, grad_weight, grad_bias, stream);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
-// Parameters are float or of the type of the vectors.
-#define MG_FOR_NORM(dtype, param, FN, ...)                                   \
-  switch (dtype) {                                                           \
-    case MG_FLOAT32: return FN(float, float, __VA_ARGS__);                   \
-    case MG_FLOAT16:                                                         \
-      if (param == MG_FLOAT32) return FN(Half, float, __VA_ARGS__);          \
-      return FN(Half, Half, __VA_ARGS__);                                    \
-    case MG_BFLOAT16:                                                        \
-      if (param == MG_FLOAT32) return FN(Bfloat16, float, __VA_ARGS__);      \
-      return FN(Bfloat16, Bfloat16, __VA_ARGS__);                            \
-  }                                                                          \
-  return hipErrorInvalidValue
-
 size_t norm_backward_workspace_bytes(int nrows, int channels) {
-  return (size_t)norm_parts(nrows) * 2 * channels * sizeof(float);
+  // (a team of one row at a time has the most workgroups)
+  return (size_t)norm_parts(nrows, 1) * 2 * channels * sizeof(float);
 }
+
+#define MG_FOR_TYPE(dtype, FN)                \
+  switch (dtype) {                            \
+    case MG_FLOAT32: return FN(float);        \
+    case MG_FLOAT16: return FN(Half);         \
+    case MG_BFLOAT16: return FN(Bfloat16);    \
+  }                                           \
+  return hipErrorInvalidValue
 
 hipError_t launch_norm(const NormArg& a, const void* x, const void* bias, void* out, float* means,
                        float* rstds, hipStream_t stream) {
-#define MG_CALL(T, P, ...) norm<T, P>(__VA_ARGS__)
-  MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL, a, x, bias, out, means, rstds, stream);
+#define MG_CALL(T) norm<T, false>(a, TokenArg(), 1.f, x, bias, DropArg(), out, means, rstds, stream)
+  MG_FOR_TYPE(a.dtype, MG_CALL);
+#undef MG_CALL
+}
+
+hipError_t launch_encode(const TokenArg& t, const NormArg& a, const void* table, float scale,
+                         const void* bias, const DropArg& drop, void* out, hipStream_t stream) {
+#define MG_CALL(T) norm<T, true>(a, t, scale, table, bias, drop, out, nullptr, nullptr, stream)
+  MG_FOR_TYPE(a.dtype, MG_CALL);
 #undef MG_CALL
 }
 
@@ -240,36 +498,21 @@ hipError_t launch_norm_backward(const NormArg& a, const void* grad, const void* 
                                 const float* means, const float* rstds, void* grad_x,
                                 void* grad_weight, void* grad_bias, void* workspace,
                                 hipStream_t stream) {
-#define MG_CALL(T, P, ...) norm_backward<T, P, T>(__VA_ARGS__)
-  MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL, a, grad, x, 1.f, means, rstds, grad_x, grad_weight,
-              grad_bias, workspace, stream);
+#define MG_CALL(T)                                                                              \
+  norm_backward<T, T, false>(a, grad, x, 1.f, means, rstds, grad_x, grad_weight, grad_bias, workspace, \
+                             stream)
+  MG_FOR_TYPE(a.dtype, MG_CALL);
 #undef MG_CALL
 }
 
 hipError_t launch_table_norm_backward(const NormArg& a, const float* sums, const void* table,
                                       float scale, void* grad_table, void* grad_weight,
                                       void* grad_bias, void* workspace, hipStream_t stream) {
-#define MG_CALL(T, P, ...) norm_backward<T, P, float>(__VA_ARGS__)
-  MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL, a, sums, table, scale, (const float*)nullptr,
-              (const float*)nullptr, grad_table, grad_weight, grad_bias, workspace, stream);
+#define MG_CALL(T)                                                                            \
+  norm_backward<T, float, true>(a, sums, table, scale, nullptr, nullptr, grad_table, grad_weight,    \
+                                grad_bias, workspace, stream)
+  MG_FOR_TYPE(a.dtype, MG_CALL);
 #undef MG_CALL
-}
-
-hipError_t launch_encode(const TokenArg& t, const NormArg& a, const void* table, float scale,
-                         const void* bias, const DropArg& drop, void* out, hipStream_t stream) {
-#define MG_CALL_F(T, P, ...) encode<T, P, float>(__VA_ARGS__)
-#define MG_CALL_I(T, P, ...) encode<T, P, int32_t>(__VA_ARGS__)
-#define MG_CALL_L(T, P, ...) encode<T, P, int64_t>(__VA_ARGS__)
-  if (t.index_kind == MG_INDEX_FLOAT32) {
-    MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL_F, t, a, table, scale, bias, drop, out, stream);
-  }
-  if (t.index_kind == MG_INDEX_INT32) {
-    MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL_I, t, a, table, scale, bias, drop, out, stream);
-  }
-  MG_FOR_NORM(a.dtype, a.param_dtype, MG_CALL_L, t, a, table, scale, bias, drop, out, stream);
-#undef MG_CALL_F
-#undef MG_CALL_I
-#undef MG_CALL_L
 }
 
 }  // namespace mg
