@@ -336,7 +336,10 @@ int mg_widen(const float* src, double* dst, size_t n, void* stream);
  * MG_FLOAT32 or equal to dtype.  Index kinds: a float index counts as the whole
  * number below it, as in mg_forward_index; an index below 0, at or beyond nrows,
  * or not-a-number names no row.  Array pointers are aligned to their elements
- * (MG_ERR_INVALID_ARGUMENT otherwise), workspaces to 256 bytes. */
+ * (MG_ERR_INVALID_ARGUMENT otherwise), workspaces to 256 bytes.  Up to 1,048,576
+ * channels (MG_ERR_UNSUPPORTED beyond).  Sums over tokens or rows are float, in
+ * an order that the sizes, the indices and the arrays' alignment alone decide:
+ * the same call gives the same bits. */
 enum { MG_FLOAT32 = 0, MG_FLOAT16 = 1, MG_BFLOAT16 = 2 };
 enum { MG_INDEX_FLOAT32 = 0, MG_INDEX_INT32 = 1, MG_INDEX_INT64 = 2 };
 
@@ -350,9 +353,8 @@ int mg_embed_types(int ntokens, int nrows, int channels, int dtype, int index_ki
 
 /* Gradients of mg_embed_types for the upstream gradient `grad`
  * [ntokens, channels]:
- *   grad_table [nrows, channels]: sum of s_n * grad[n,:] over the tokens of a row, in float and
- *     in an order that the sizes and indices alone decide (the same call gives the same bits);
- *     rows without tokens get zero
+ *   grad_table [nrows, channels]: sum of s_n * grad[n,:] over the tokens of a row; rows without
+ *     tokens get zero
  *   grad_scales [ntokens] float32: sum over the channels of grad[n,:] * table[type_index[n],:]
  * Either may be NULL; `table` is read for grad_scales only. */
 size_t mg_embed_types_backward_workspace_size(int ntokens, int nrows, int channels);
@@ -371,9 +373,8 @@ int mg_layer_norm(int nrows, int channels, int dtype, int param_dtype, const voi
                   float* rstd, void* stream);
 
 /* Gradients of mg_layer_norm: grad_x [nrows, channels], grad_weight and
- * grad_bias [channels] of param_dtype, each of which may be NULL.  The sums over
- * the rows are float, in an order that the sizes alone decide.  grad_x == grad
- * is not allowed. */
+ * grad_bias [channels] of param_dtype, each of which may be NULL.  grad_x must
+ * be neither grad nor x. */
 size_t mg_layer_norm_backward_workspace_size(int nrows, int channels);
 int mg_layer_norm_backward(int nrows, int channels, int dtype, int param_dtype, const void* grad,
                            const void* x, const float* mean, const float* rstd,
@@ -403,7 +404,7 @@ int mg_encode_types(int ntokens, int nrows, int channels, int dtype, int param_d
 /* Gradients of mg_encode_types: grad_table [nrows, channels], grad_weight and
  * grad_bias [channels]; each may be NULL.  All tokens of a row share its
  * normed vector and the norm's backward pass is linear in the gradient, so the
- * gradients of a row's tokens are summed first (float, fixed order). */
+ * gradients of a row's tokens are summed first. */
 size_t mg_encode_types_backward_workspace_size(int ntokens, int nrows, int channels);
 int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, int param_dtype,
                              int index_kind, const void* type_index, const void* grad,

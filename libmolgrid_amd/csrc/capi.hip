@@ -87,8 +87,11 @@ bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(
 size_t dtype_size(int dtype) { return dtype == MG_FLOAT32 ? 4 : 2; }
 size_t index_size(int kind) { return kind == MG_INDEX_INT64 ? 8 : 4; }
 
+constexpr int kMaxVectorChannels = 1 << 20;   // (launches have a workgroup for every 64 of them)
+
 int check_tokens(const TokenArg& t) {
   if (t.ntokens < 0 || t.nrows < 0 || t.channels < 0) return MG_ERR_INVALID_ARGUMENT;
+  if (t.channels > kMaxVectorChannels) return MG_ERR_UNSUPPORTED;
   if (!is_dtype(t.dtype)) return MG_ERR_INVALID_ARGUMENT;
   if (t.index_kind < MG_INDEX_FLOAT32 || t.index_kind > MG_INDEX_INT64) return MG_ERR_INVALID_ARGUMENT;
   if (!aligned(t.index, index_size(t.index_kind))) return MG_ERR_INVALID_ARGUMENT;
@@ -96,6 +99,7 @@ int check_tokens(const TokenArg& t) {
 }
 int check_norm(const NormArg& a) {
   if (a.nrows < 0 || a.channels < 0) return MG_ERR_INVALID_ARGUMENT;
+  if (a.channels > kMaxVectorChannels) return MG_ERR_UNSUPPORTED;
   if (!is_dtype(a.dtype) || (a.param_dtype != MG_FLOAT32 && a.param_dtype != a.dtype))
     return MG_ERR_INVALID_ARGUMENT;
   if (!(a.eps >= 0.f)) return MG_ERR_INVALID_ARGUMENT;
@@ -706,7 +710,7 @@ int mg_embed_types_backward(int ntokens, int nrows, int channels, int dtype, int
                          mg_embed_types_backward_workspace_size(ntokens, nrows, channels));
     if (rc != MG_OK) return rc;
     rc = from_hip(launch_embed_backward(t, grad, scale, scales, grad_table, workspace,
-                                        workspace_bytes, (hipStream_t)stream));
+                                        (hipStream_t)stream));
     if (rc != MG_OK) return rc;
   }
   if (to_scales)
@@ -837,8 +841,7 @@ int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, in
   const size_t sums_bytes = ((size_t)nrows * channels * sizeof(float) + 255) / 256 * 256;
   void* rest = nrows > 0 ? static_cast<char*>(workspace) + sums_bytes : nullptr;
   if (nrows > 0) {
-    rc = from_hip(launch_row_sums(t, grad, drop, sums, rest, workspace_bytes - sums_bytes,
-                                  (hipStream_t)stream));
+    rc = from_hip(launch_row_sums(t, grad, drop, sums, rest, (hipStream_t)stream));
     if (rc != MG_OK) return rc;
   }
   return from_hip(launch_table_norm_backward(a, sums, table, scale, grad_table, grad_weight,

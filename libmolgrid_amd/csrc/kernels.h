@@ -125,9 +125,9 @@ hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const
 size_t row_sums_workspace_bytes(int ntokens, int nrows, int channels);
 hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scale,
                                  const float* scales, void* grad_table, void* workspace,
-                                 size_t workspace_bytes, hipStream_t stream);
+                                 hipStream_t stream);
 hipError_t launch_row_sums(const TokenArg& t, const void* grad, const DropArg& drop, float* out,
-                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+                           void* workspace, hipStream_t stream);
 hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
                                  float* grad_scales, hipStream_t stream);
 
