@@ -683,7 +683,7 @@ int mg_embed_types(int ntokens, int nrows, int channels, int dtype, int index_ki
 
 size_t mg_embed_types_backward_workspace_size(int ntokens, int nrows, int channels) {
   if (ntokens <= 0 || nrows <= 0 || channels <= 0) return 0;
-  return row_sums_workspace_bytes(ntokens, nrows, channels);
+  return embed_backward_workspace_bytes(ntokens, nrows, channels);
 }
 
 int mg_embed_types_backward(int ntokens, int nrows, int channels, int dtype, int index_kind,
@@ -801,13 +801,9 @@ int mg_encode_types(int ntokens, int nrows, int channels, int dtype, int param_d
   return from_hip(launch_encode(t, a, table, scale, bias, drop, out, (hipStream_t)stream));
 }
 
-// The sums over every row's tokens come first in the workspace, then what either step needs.
 size_t mg_encode_types_backward_workspace_size(int ntokens, int nrows, int channels) {
-  if (nrows <= 0 || channels <= 0) return 0;
-  const size_t sums = ((size_t)nrows * channels * sizeof(float) + 255) / 256 * 256;
-  const size_t tokens = ntokens > 0 ? row_sums_workspace_bytes(ntokens, nrows, channels) : 0;
-  const size_t norm = norm_backward_workspace_bytes(nrows, channels);
-  return sums + (tokens > norm ? tokens : norm);
+  if (ntokens < 0 || nrows <= 0 || channels <= 0) return 0;
+  return encode_backward_workspace_bytes(ntokens, nrows, channels);
 }
 
 int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, int param_dtype,
@@ -837,15 +833,8 @@ int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, in
                          mg_encode_types_backward_workspace_size(ntokens, nrows, channels));
     if (rc != MG_OK) return rc;
   }
-  float* sums = static_cast<float*>(workspace);
-  const size_t sums_bytes = ((size_t)nrows * channels * sizeof(float) + 255) / 256 * 256;
-  void* rest = nrows > 0 ? static_cast<char*>(workspace) + sums_bytes : nullptr;
-  if (nrows > 0) {
-    rc = from_hip(launch_row_sums(t, grad, drop, sums, rest, (hipStream_t)stream));
-    if (rc != MG_OK) return rc;
-  }
-  return from_hip(launch_table_norm_backward(a, sums, table, scale, grad_table, grad_weight,
-                                             grad_bias, rest, (hipStream_t)stream));
+  return from_hip(launch_encode_backward(t, a, grad, table, scale, drop, grad_table, grad_weight,
+                                         grad_bias, workspace, (hipStream_t)stream));
 }
 
 }  // extern "C"

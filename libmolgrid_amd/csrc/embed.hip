@@ -132,22 +132,24 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T*
   const uint32_t end = min(begin + (uint32_t)share, (uint32_t)t.ntokens);
   if (c < t.channels)
     for (uint32_t n0 = begin + team; n0 < end; n0 += teams * kTableUnroll) {
+      uint32_t n[kTableUnroll];
       int row[kTableUnroll];
       float by[kTableUnroll], g[kTableUnroll][VEC];
 #pragma unroll
-      for (int u = 0; u < kTableUnroll; ++u) {
-        const uint32_t n = n0 + u * teams;
-        row[u] = n < end ? token_row(t, n) : -1;
-        by[u] = a.scales && n < end ? a.scales[n] : a.scale;
-        if (n < end) load_floats<T, VEC>(grad + (size_t)n * t.channels + c, g[u]);
-      }
+      for (int u = 0; u < kTableUnroll; ++u) n[u] = n0 + u * teams;
+      token_rows(t, n, end, row);
+#pragma unroll
+      for (int u = 0; u < kTableUnroll; ++u) by[u] = a.scales && n[u] < end ? a.scales[n[u]] : a.scale;
+#pragma unroll
+      for (int u = 0; u < kTableUnroll; ++u)
+        if (n[u] < end) load_floats<T, VEC>(grad + (size_t)n[u] * t.channels + c, g[u]);
 #pragma unroll
       for (int u = 0; u < kTableUnroll; ++u) {
         if (row[u] < 0) continue;
         float sum[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] = mine[(row[u] * VEC + i) * LANES];
-        add_token<DROP, VEC>((size_t)(n0 + u * teams) * t.channels + c, a, by[u], seed, offset, g[u], sum);
+        add_token<DROP, VEC>((size_t)n[u] * t.channels + c, a, by[u], seed, offset, g[u], sum);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) mine[(row[u] * VEC + i) * LANES] = sum[i];
       }
@@ -191,14 +193,36 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
 
 // ---- any table: the tokens sorted by row ----------------------------------------------------------
 //
-// One launch sorts: a workgroup owns a range of rows, reads every index twice and keeps those of its
-// range.  First it counts its rows' tokens, and the tokens of lower rows, which is where its part of
-// the order begins; then it writes its tokens in place.  Each of its waves goes through a piece of
-// the tokens of its own, with counters of its own, so the order within a row is that of the
-// tokens.  All workgroups read all indices (out of the L2 after the first), which costs less than
-// the launches of a sort by digits for up to about 2^18 tokens.
+// One launch sorts: a workgroup owns a range of rows, reads every index and keeps those of its range.
+// First it counts its rows' tokens, and the tokens of lower rows, which is where its part of the
+// order begins; then it goes again through the steps of 64 tokens that held one of its own and writes
+// those in place.  Each of its waves goes through a piece of the tokens of its own, with counters of
+// its own, so the order within a row is that of the tokens.  All workgroups read all indices (out of
+// the L2 after the first), which costs less than the launches of a sort by digits for up to about
+// 2^18 tokens.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kSortRange = 960;   // most rows of a workgroup: 60 KB of counters
+
+// A row of up to kDirect tokens is added up by one team.  Longer ones are cut into pieces that
+// start at multiples of their length from the row's start: about as many pieces as a piece has
+// tokens, a multiple of kBlock.  A piece's sum has slot 2 b + f, where b is the block of kBlock
+// positions of the order that the piece starts in and f whether it is its row's first: of a block's
+// positions at most two start pieces, a first one (its row then holds the block's last position) and
+// a later one (its row then holds the block's first position).
+constexpr int kBlock = 32, kDirect = 64;
+
+__device__ __forceinline__ int piece_length(int count) {
+  return ((int)sqrtf((float)count) / kBlock + 1) * kBlock;
+}
+__device__ __forceinline__ int piece_slot(int from, int length, int j) {
+  return (from + j * length) / kBlock * 2 + (j == 0 ? 1 : 0);
+}
+
+struct Sorted {
+  int32_t* start;      // [nrows + 1]: where a row's tokens begin in order
+  int32_t* order;      // [ntokens]
+  int32_t* piece_row;  // [2 blocks]: row of the piece in a slot, or -1 (unwritten past the last token)
+};
 
 __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
 #pragma unroll
@@ -209,33 +233,37 @@ __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
   return v;
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(TokenArg t, int range,
-                                                                   int32_t* __restrict__ start,
-                                                                   int32_t* __restrict__ order) {
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __restrict__ index,
+                                                                   uint32_t ntokens, int nrows,
+                                                                   int range, Sorted sorted) {
   HIP_DYNAMIC_SHARED(int, count);   // [kSortWaves][range]
   __shared__ int sums[kSortWaves];
+  __shared__ int last;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int row0 = blockIdx.x * range, rows = min(range, t.nrows - row0);
+  const int row0 = blockIdx.x * range, rows = min(range, nrows - row0);
   for (int i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) count[i] = 0;
   __syncthreads();
-  const uint32_t ntokens = (uint32_t)t.ntokens;
-  const uint32_t piece = (ntokens + kSortThreads - 1) / kSortThreads * kWave;
-  const uint32_t begin = wave * piece, end = min(begin + piece, ntokens);
+  const uint32_t steps = (ntokens + kSortThreads - 1) / kSortThreads;   // of 64 tokens, for each wave
+  const uint32_t begin = wave * steps * kWave;
+  const uint32_t end = ntokens < begin + steps * kWave ? ntokens : begin + steps * kWave;
   int* mine = count + wave * range;
   constexpr int kAhead = 8;   // indices of a lane in flight
+  const auto fetch = [&](uint32_t n) { return n < end ? table_row(index[n], nrows) : -1; };
   int lower = 0;
-  for (uint32_t n0 = begin; n0 < end; n0 += kAhead * kWave) {
+  uint64_t held = 0;   // bit b of lane l: step 64 l + b has a token of this workgroup's rows
+  for (uint32_t s0 = 0; s0 < steps; s0 += kAhead) {
     int row[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t n = n0 + u * kWave + lane;
-      row[u] = n < end ? token_row(t, n) : -1;
-    }
+    for (int u = 0; u < kAhead; ++u) row[u] = fetch(begin + (s0 + u) * kWave + lane);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       lower += row[u] >= 0 && row[u] < row0 ? 1 : 0;
       const int r = row[u] - row0;
-      if (row[u] >= row0 && r < rows) atomicAdd(&mine[r], 1);
+      const bool inside = row[u] >= row0 && r < rows;
+      if (inside) atomicAdd(&mine[r], 1);
+      const uint32_t s = s0 + u;
+      if (__ballot(inside) && (uint32_t)lane == s / 64) held |= (uint64_t)1 << (s % 64);
     }
   }
   lower = wave_inclusive_sum(lower, lane);
@@ -245,78 +273,103 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(TokenArg t, i
   for (int w = 0; w < kSortWaves; ++w) base += sums[w];
   __syncthreads();
   // where the tokens of every row, and of every wave in it, begin
-  const int per_thread = (range + kSortThreads - 1) / kSortThreads;
-  const int r0 = threadIdx.x * per_thread, r1 = min(r0 + per_thread, rows);
+  const int r = threadIdx.x;   // (a row a thread: a range has fewer rows than a workgroup threads)
   int total = 0;
-  for (int r = r0; r < r1; ++r)
+  if (r < rows)
     for (int w = 0; w < kSortWaves; ++w) total += count[w * range + r];
   const int through = wave_inclusive_sum(total, lane);
   if (lane == kWave - 1) sums[wave] = through;
   __syncthreads();
   int at = base + through - total;
   for (int w = 0; w < wave; ++w) at += sums[w];
-  for (int r = r0; r < r1; ++r) {
-    start[row0 + r] = at;
+  if (r < rows) {
+    sorted.start[row0 + r] = at;
     for (int w = 0; w < kSortWaves; ++w) {
       const int c = count[w * range + r];
       count[w * range + r] = at;
       at += c;
     }
-    if (row0 + r == t.nrows - 1) start[t.nrows] = at;
+    if (r == rows - 1) last = at;
+    if (row0 + r == nrows - 1) sorted.start[nrows] = at;
   }
   __syncthreads();
-  const unsigned long long below = (1ull << lane) - 1;
-  for (uint32_t n0 = begin; n0 < end; n0 += kAhead * kWave) {
-    int row[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t n = n0 + u * kWave + lane;
-      row[u] = n < end ? token_row(t, n) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int r = row[u] - row0;
-      const bool inside = row[u] >= row0 && r < rows;
-      unsigned long long left = __ballot(inside);
-      while (left) {   // one turn for each row among the wave's tokens
-        const int first = __builtin_amdgcn_readlane(r, (int)__builtin_ctzll(left));
-        const unsigned long long same = __ballot(inside && r == first);
-        const int to = mine[first];
-        wave_lds_fence();
-        if (inside && r == first) {
-          const int rank = __popcll(same & below);
-          order[to + rank] = (int32_t)(n0 + u * kWave + lane);
-          if (rank == 0) mine[first] = to + __popcll(same);
+  // slots of the blocks of the order that this workgroup's rows hold the first or last position of
+  if (sorted.piece_row)
+    for (int i = wave; i < rows; i += kSortWaves) {
+      const int from = count[i], to = i + 1 < rows ? count[i + 1] : last;
+      const bool cut = to - from > kDirect;
+      const int length = piece_length(to - from);
+      for (int b = from / kBlock + lane; b * kBlock < to; b += kWave) {
+        const int first = b * kBlock;
+        if (first >= from) {
+          const int j = (first - from + length - 1) / length, p = from + j * length;
+          sorted.piece_row[2 * b] = cut && j > 0 && p < to && p < first + kBlock ? row0 + i : -1;
         }
-        wave_lds_fence();
-        left &= ~same;
+        if (first + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = cut && first <= from ? row0 + i : -1;
       }
+    }
+  __syncthreads();
+  const unsigned long long below = (1ull << lane) - 1;
+  const auto place = [&](uint32_t n, int row) {
+    const int r = row - row0;
+    const bool inside = row >= row0 && r < rows;
+    unsigned long long left = __ballot(inside);
+    while (left) {   // one turn for each row among the wave's tokens
+      const int first = __builtin_amdgcn_readlane(r, (int)__builtin_ctzll(left));
+      const unsigned long long same = __ballot(inside && r == first);
+      const int to = mine[first];
+      wave_lds_fence();
+      if (inside && r == first) {
+        const int rank = __popcll(same & below);
+        sorted.order[to + rank] = (int32_t)n;
+        if (rank == 0) mine[first] = to + __popcll(same);
+      }
+      wave_lds_fence();
+      left &= ~same;
+    }
+  };
+  constexpr int kTogether = 4;
+  if (steps > 64 * kWave) {   // (more than four million tokens: more steps than bits)
+    for (uint32_t s = 0; s < steps; ++s) {
+      const uint32_t n = begin + s * kWave + lane;
+      place(n, fetch(n));
+    }
+    return;
+  }
+  for (uint32_t l = 0; l * 64 < steps; ++l) {
+    uint64_t bits = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)held, (int)l) |
+                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(held >> 32), (int)l) << 32;
+    while (bits) {
+      uint32_t n[kTogether];
+      int row[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const uint32_t s = bits ? l * 64 + (uint32_t)__builtin_ctzll(bits) : steps;
+        bits &= bits - 1;
+        n[u] = begin + s * kWave + lane;
+        row[u] = s < steps ? fetch(n[u]) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) place(n[u], row[u]);
     }
   }
 }
-
-// Tokens of a row that one team adds; rows of more are cut where the order's multiples of it are.
-constexpr int kPiece = 128;
-
-struct Sorted {
-  const int32_t* start;   // [nrows + 1]: where a row's tokens begin in order
-  const int32_t* order;
-};
 
 // Adds the tokens order[begin .. end) to acc, in that order.
 template <typename T, int VEC, int LANES, int K, bool DROP>
 __device__ __forceinline__ void add_tokens(const TokenArg& t, const T* grad, const SumArg& a,
                                            const int32_t* order, int begin, int end, int lane,
                                            uint64_t seed, uint64_t offset, float (&acc)[K][VEC]) {
-  constexpr int kAhead = K * VEC <= 8 ? 4 : 2;
+  constexpr int kAhead = K == 1 ? 8 : K <= 4 ? 4 : 2;
   for (int i0 = begin; i0 < end; i0 += kAhead) {
     RowPacks<T, VEC, K> g[kAhead];
     uint32_t n[kAhead];
     float by[kAhead];
 #pragma unroll
+    for (int u = 0; u < kAhead; ++u) n[u] = i0 + u < end ? (uint32_t)order[i0 + u] : 0;
+#pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const bool live = i0 + u < end;
-      n[u] = live ? (uint32_t)order[i0 + u] : 0;
       by[u] = !live ? 0.f : a.scales ? a.scales[n[u]] : a.scale;
       load_row<T, VEC, LANES, K>(grad + (size_t)n[u] * t.channels, t.channels, lane, live, g[u]);
     }
@@ -344,79 +397,126 @@ __device__ __forceinline__ void store_row(O* to, int channels, int lane, const f
   }
 }
 
-// The first `piece_blocks` workgroups take pieces of long rows, whose sums go to `partial`
-// (piece i: the row that its first token is of, then the row that its last one is of), the others
-// rows.
-template <typename T, typename O, int VEC, int LANES, int K, bool DROP>
-__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void sorted_rows_kernel(
-    TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted, int piece_blocks,
-    O* __restrict__ out, float* __restrict__ partial) {
-  using Shape = TeamShape<LANES, K>;
-  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+// The pieces of long rows, a team a slot.
+template <typename T, int VEC, int LANES, int K, bool DROP>
+__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void pieces_kernel(
+    TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted, float* __restrict__ partial) {
+  const int lane = threadIdx.x % LANES;
+  const int slot = blockIdx.x * TeamShape<LANES, K>::TEAMS + threadIdx.x / LANES;
+  const int block = slot / 2;
+  if ((int64_t)block * kBlock + (slot & 1 ? kBlock - 1 : 0) >= sorted.start[t.nrows]) return;
+  const int row = sorted.piece_row[slot];
+  if (row < 0) return;
   uint64_t seed = 0, offset = 0;
   if (DROP) drop_key(a.drop, seed, offset);
-  const int blocks = gridDim.x - piece_blocks;
-  if ((int)blockIdx.x < piece_blocks) {
-    const int total = sorted.start[t.nrows];
-    const int i = blockIdx.x * Shape::TEAMS + team;
-    if (i > (total - 1) / kPiece || total == 0) return;
-    const int begin = i * kPiece, end = total - begin < kPiece ? total : begin + kPiece;
-    const int first = token_row(t, (uint32_t)sorted.order[begin]);
-    const int last = token_row(t, (uint32_t)sorted.order[end - 1]);
-    for (int which = 0; which < (first == last ? 1 : 2); ++which) {
-      const int row = which ? last : first;
-      const int from = sorted.start[row], to = sorted.start[row + 1];
-      if (to - from <= kPiece) continue;
-      float acc[K][VEC] = {};
-      add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, max(from, begin), min(to, end), lane,
-                                         seed, offset, acc);
-      store_row<float, VEC, LANES, K>(partial + ((size_t)i * 2 + which) * t.channels, t.channels, lane, acc);
-    }
-    return;
-  }
-  for (uint32_t row = (blockIdx.x - piece_blocks) * Shape::TEAMS + team; row < (uint32_t)t.nrows;
-       row += blocks * Shape::TEAMS) {
-    const int from = sorted.start[row], to = sorted.start[row + 1];
-    if (to - from > kPiece) continue;
-    float acc[K][VEC] = {};
-    add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, from, to, lane, seed, offset, acc);
-    store_row<O, VEC, LANES, K>(out + (size_t)row * t.channels, t.channels, lane, acc);
-  }
+  const int from = sorted.start[row], to = sorted.start[row + 1], length = piece_length(to - from);
+  const int j = slot & 1 ? 0 : (block * kBlock - from + length - 1) / length;
+  const int begin = from + j * length, end = min(begin + length, to);
+  float acc[K][VEC] = {};
+  add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, begin, end, lane, seed, offset, acc);
+  store_row<float, VEC, LANES, K>(partial + (size_t)slot * t.channels, t.channels, lane, acc);
 }
 
-// Long rows: the workgroup of the piece that such a row begins in adds the row's pieces, a wave
-// every fourth one.
-template <typename O>
-__global__ __launch_bounds__(kThreads) void long_rows_kernel(TokenArg t, Sorted sorted,
-                                                             const float* __restrict__ partial,
-                                                             O* __restrict__ out) {
-  constexpr int kWaves = kThreads / kWave;
-  __shared__ float sums[kWaves][kWave];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int total = sorted.start[t.nrows];
-  const int piece = blockIdx.x, begin = piece * kPiece;
-  if (begin >= total) return;
-  const int end = total - begin < kPiece ? total : begin + kPiece;
-  const int row = token_row(t, (uint32_t)sorted.order[end - 1]);
-  const int from = sorted.start[row], to = sorted.start[row + 1];
-  if (to - from <= kPiece || from < begin) return;
-  const int last = (to - 1) / kPiece;
-  const int first_slot = from > begin ? 1 : 0;   // behind another row in its first piece
-  for (int c0 = 0; c0 < t.channels; c0 += kWave) {
-    const int c = c0 + lane;
-    float sum = 0.f;
-    if (c < t.channels)
-#pragma unroll 4
-      for (int i = piece + wave; i <= last; i += kWaves)
-        sum += partial[((size_t)i * 2 + (i == piece ? first_slot : 0)) * t.channels + c];
-    lds_barrier();
-    sums[wave][lane] = sum;
-    lds_barrier();
-    if (wave == 0 && c < t.channels) {
-      for (int w = 1; w < kWaves; ++w) sum += sums[w][lane];
-      out[(size_t)row * t.channels + c] = narrow<O>(sum);
-    }
+// What a row's sum goes through when the vectors were normed rows of the scaled table
+struct TableNorm {
+  const void* table;
+  float scale;
+  NormArg norm;
+  bool to_table, to_params;
+  ParamSums params;
+};
+
+// Every row of the table: the sum of its tokens, or of its pieces.  The bounds of a team's next row
+// are read ahead.  NORM: the sum is the gradient of the row's normed vector, which is taken back
+// through the norm while it is here; the workgroups then stay, and their teams' shares of the
+// gradients of weight and bias are added up at the end.
+template <typename T, int VEC, int LANES, int K, bool DROP, bool NORM>
+__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
+    TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted,
+    const float* __restrict__ partial, T* __restrict__ out, TableNorm norm) {
+  using Shape = TeamShape<LANES, K>;
+  __shared__ float slots[3][2 * Shape::WAVES];
+  HIP_DYNAMIC_SHARED(float, param_sums);
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  const int channels = t.channels;
+  const uint32_t nrows = (uint32_t)t.nrows, step = gridDim.x * Shape::TEAMS;
+  uint64_t seed = 0, offset = 0;
+  if (DROP) drop_key(a.drop, seed, offset);
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+  if (NORM) {
+    load_param<T, VEC, LANES, K>(norm.norm.weight, norm.params.is_float, 1.f, channels, lane, w);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.f;
   }
+  const uint32_t mine = blockIdx.x * Shape::TEAMS + team;
+  int next_from = mine < nrows ? sorted.start[mine] : 0, next_to = mine < nrows ? sorted.start[mine + 1] : 0;
+  for (uint32_t row0 = blockIdx.x * Shape::TEAMS; row0 < nrows; row0 += step) {
+    const uint32_t row = row0 + team;
+    const int from = next_from, to = next_to;
+    const bool more = row + step < nrows;
+    next_from = more ? sorted.start[row + step] : 0;
+    next_to = more ? sorted.start[row + step + 1] : 0;
+    const bool some = to > from;
+    float v[K][VEC] = {};
+    RowPacks<T, VEC, K> x;
+    if (NORM)
+      load_row<T, VEC, LANES, K>(static_cast<const T*>(norm.table) + (some ? (size_t)row * channels : 0),
+                                 channels, lane, some, x);
+    if (to - from <= kDirect) {
+      add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, from, to, lane, seed, offset, v);
+    } else {
+      const int length = piece_length(to - from), pieces = (to - from + length - 1) / length;
+      constexpr int kAhead = K == 1 ? 8 : K <= 4 ? 4 : 2;
+      for (int j0 = 0; j0 < pieces; j0 += kAhead) {
+        RowPacks<float, VEC, K> p[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          load_row<float, VEC, LANES, K>(
+              partial + (j0 + u < pieces ? (size_t)piece_slot(from, length, j0 + u) * channels : 0), channels,
+              lane, j0 + u < pieces, p[u]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[k][i] += p[u].pack[k].v[i];
+      }
+    }
+    // (all teams of a wave come along, and a team of several waves is a workgroup)
+    if (NORM && __ballot(some)) {
+      float h[K][VEC];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[k][i] = norm.scale * widen(x.pack[k].v[i]);
+      float mean, rstd;
+      team_stats<VEC, LANES, K>(h, channels, lane, norm.norm.eps, slots[0], slots[1], mean, rstd);
+      float both[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          h[k][i] *= rstd;
+          const float q = v[k][i] * w[k][i];
+          both[0] += q;
+          both[1] = fmaf(q, h[k][i], both[1]);
+          if (some) dw[k][i] = fmaf(v[k][i], h[k][i], dw[k][i]);
+          db[k][i] += v[k][i];
+        }
+      team_sums<LANES>(both, slots[2]);
+      const float mean_q = both[0] / channels, mean_qh = both[1] / channels;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          v[k][i] = some ? norm.scale * rstd * (v[k][i] * w[k][i] - mean_q - h[k][i] * mean_qh) : 0.f;
+    }
+    if (row < nrows && (!NORM || norm.to_table))
+      store_row<T, VEC, LANES, K>(out + (size_t)row * channels, channels, lane, v);
+  }
+  if (NORM && norm.to_params) add_up_params<T, VEC, LANES, K>(dw, db, lane, channels, param_sums, norm.params);
 }
 
 // Rows wider than any team: a workgroup a row, a thread a channel.
@@ -522,16 +622,16 @@ size_t few_rows_bytes(int ntokens, int nrows, int channels) {
 }
 
 struct SortedLayout {
-  size_t start, order, partial, bytes;   // offsets into the workspace
-  int pieces;
+  size_t order, piece_row, partial, bytes;   // offsets into the workspace; start is first
+  int slots;
 };
 SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   SortedLayout l;
-  l.start = 0;
+  l.slots = ntokens > kDirect ? (ntokens + kBlock - 1) / kBlock * 2 : 0;
   l.order = round_up(((size_t)nrows + 1) * sizeof(int32_t));
-  l.partial = l.order + round_up((size_t)ntokens * sizeof(int32_t));
-  l.pieces = ntokens > kPiece ? (ntokens + kPiece - 1) / kPiece : 0;
-  l.bytes = l.partial + round_up((size_t)l.pieces * 2 * channels * sizeof(float));
+  l.piece_row = l.order + round_up((size_t)ntokens * sizeof(int32_t));
+  l.partial = l.piece_row + round_up((size_t)l.slots * sizeof(int32_t));
+  l.bytes = l.partial + (channels <= kMostTeamChannels ? round_up((size_t)l.slots * channels * sizeof(float)) : 0);
   return l;
 }
 
@@ -558,38 +658,65 @@ hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, void* 
   return hipGetLastError();
 }
 
-template <typename T, typename O, bool DROP>
-hipError_t row_sums(const TokenArg& t, const void* grad, const SumArg& a, void* out, void* workspace,
-                    hipStream_t stream) {
-  if (t.nrows <= kFewRows) return few_rows<T, O, DROP>(t, grad, a, out, (float*)workspace, stream);
-  const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
-  char* base = static_cast<char*>(workspace);
-  int32_t* start = reinterpret_cast<int32_t*>(base + l.start);
-  int32_t* order = reinterpret_cast<int32_t*>(base + l.order);
-  float* partial = reinterpret_cast<float*>(base + l.partial);
+void sort_tokens(const TokenArg& t, const Sorted& sorted, hipStream_t stream) {
   int range = (t.nrows + 255) / 256;
   if (range > kSortRange) range = kSortRange;
-  hipLaunchKernelGGL(sort_tokens_kernel, dim3((t.nrows + range - 1) / range), dim3(kSortThreads),
-                     (size_t)kSortWaves * range * sizeof(int), stream, t, range, start, order);
-  const Sorted sorted{start, order};
-  bool done = false;
-  with_packs_of<T>(t.channels, address(grad) | address(out), [&](auto vec) {
+  const dim3 grid((t.nrows + range - 1) / range), block(kSortThreads);
+  const size_t shared = (size_t)kSortWaves * range * sizeof(int);
+  if (t.index_kind == MG_INDEX_FLOAT32)
+    hipLaunchKernelGGL(sort_tokens_kernel<float>, grid, block, shared, stream, (const float*)t.index,
+                       (uint32_t)t.ntokens, t.nrows, range, sorted);
+  else if (t.index_kind == MG_INDEX_INT32)
+    hipLaunchKernelGGL(sort_tokens_kernel<int32_t>, grid, block, shared, stream, (const int32_t*)t.index,
+                       (uint32_t)t.ntokens, t.nrows, range, sorted);
+  else
+    hipLaunchKernelGGL(sort_tokens_kernel<int64_t>, grid, block, shared, stream, (const int64_t*)t.index,
+                       (uint32_t)t.ntokens, t.nrows, range, sorted);
+}
+
+// Workgroups of rows_kernel that stay, for the sums over all rows
+constexpr int kRowParts = 1024;
+
+// The sums by row of a table of more than kFewRows rows, or (NORM) what follows from them.
+template <typename T, bool DROP, bool NORM>
+hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, void* out, void* workspace,
+                       TableNorm norm, hipStream_t stream) {
+  const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
+  char* base = static_cast<char*>(workspace);
+  float* partial = reinterpret_cast<float*>(base + l.partial);
+  Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order),
+                l.slots ? reinterpret_cast<int32_t*>(base + l.piece_row) : nullptr};
+  sort_tokens(t, sorted, stream);
+  int parts = 0;
+  with_packs_of<T>(t.channels, address(grad) | address(out) | address(NORM ? norm.table : nullptr), [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
-    done = with_team<VEC>((t.channels + VEC - 1) / VEC, [&](auto shape) {
+    with_sum_team<VEC>((t.channels + VEC - 1) / VEC, [&](auto shape) {
       using S = decltype(shape);
-      const int piece_blocks = (l.pieces + S::TEAMS - 1) / S::TEAMS;
-      const unsigned blocks = at_most(((size_t)t.nrows + S::TEAMS - 1) / S::TEAMS, kResident * 4);
-      hipLaunchKernelGGL((sorted_rows_kernel<T, O, VEC, S::LANES, S::K, DROP>),
-                         dim3(blocks + piece_blocks), dim3(S::THREADS), 0, stream, t, (const T*)grad, a,
-                         sorted, piece_blocks, (O*)out, partial);
+      if (l.slots)
+        hipLaunchKernelGGL((pieces_kernel<T, VEC, S::LANES, S::K, DROP>),
+                           dim3((l.slots + S::TEAMS - 1) / S::TEAMS), dim3(S::THREADS), 0, stream, t,
+                           (const T*)grad, a, sorted, partial);
+      parts = (int)at_most(((size_t)t.nrows + S::TEAMS - 1) / S::TEAMS, NORM ? kRowParts : 16384);
+      const size_t shared = NORM && S::LANES <= kWave ? (size_t)2 * t.channels * sizeof(float) : 0;
+      hipLaunchKernelGGL((rows_kernel<T, VEC, S::LANES, S::K, DROP, NORM>), dim3(parts), dim3(S::THREADS),
+                         shared, stream, t, (const T*)grad, a, sorted, partial, (T*)out, norm);
     });
   });
-  if (!done)
-    hipLaunchKernelGGL((wide_rows_kernel<T, O, DROP>), dim3(at_most(t.nrows, 8192), 16), dim3(kThreads), 0,
-                       stream, t, (const T*)grad, a, sorted, (O*)out);
-  else if (l.pieces > 0)
-    hipLaunchKernelGGL((long_rows_kernel<O>), dim3(l.pieces), dim3(kThreads), 0, stream, t, sorted, partial,
-                       (O*)out);
+  if (NORM && norm.to_params && parts > 1)
+    return launch_sum_partials(norm.norm, norm.params.partial, parts, norm.params.weight, norm.params.bias,
+                               stream);
+  return hipGetLastError();
+}
+
+template <typename T, typename O, bool DROP>
+hipError_t wide_rows(const TokenArg& t, const void* grad, const SumArg& a, void* out, void* workspace,
+                     hipStream_t stream) {
+  const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
+  char* base = static_cast<char*>(workspace);
+  const Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order), nullptr};
+  sort_tokens(t, sorted, stream);
+  hipLaunchKernelGGL((wide_rows_kernel<T, O, DROP>), dim3(at_most(t.nrows, 8192), 16), dim3(kThreads), 0, stream,
+                     t, (const T*)grad, a, sorted, (O*)out);
   return hipGetLastError();
 }
 
@@ -616,7 +743,8 @@ hipError_t zero(void* out, size_t n, hipStream_t stream) {
   }                                           \
   return hipErrorInvalidValue
 
-size_t row_sums_workspace_bytes(int ntokens, int nrows, int channels) {
+// A table's gradient has few rows, or rows that are too wide for a team, or is sorted.
+size_t embed_backward_workspace_bytes(int ntokens, int nrows, int channels) {
   if (nrows <= kFewRows) return few_rows_bytes(ntokens, nrows, channels);
   return sorted_layout(ntokens, nrows, channels).bytes;
 }
@@ -632,19 +760,12 @@ hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scal
                                  const float* scales, void* grad_table, void* workspace,
                                  hipStream_t stream) {
   const SumArg a{scale, scales, DropArg()};
-  const size_t elements = (size_t)t.nrows * t.channels;
-#define MG_CALL(T)                                             \
-  t.ntokens == 0 ? zero<T>(grad_table, elements, stream)       \
-                 : row_sums<T, T, false>(t, grad, a, grad_table, workspace, stream)
-  MG_FOR_TYPE(t.dtype, MG_CALL);
-#undef MG_CALL
-}
-
-hipError_t launch_row_sums(const TokenArg& t, const void* grad, const DropArg& drop, float* out,
-                           void* workspace, hipStream_t stream) {
-  const SumArg a{1.f, nullptr, drop};
-  if (t.ntokens == 0) return zero<float>(out, (size_t)t.nrows * t.channels, stream);
-#define MG_CALL(T) row_sums<T, float, true>(t, grad, a, out, workspace, stream)
+#define MG_CALL(T)                                                                                  \
+  t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)                        \
+  : t.nrows <= kFewRows ? few_rows<T, T, false>(t, grad, a, grad_table, (float*)workspace, stream)  \
+  : t.channels > kMostTeamChannels ? wide_rows<T, T, false>(t, grad, a, grad_table, workspace, stream) \
+                                   : sorted_rows<T, false, false>(t, grad, a, grad_table, workspace, \
+                                                                  TableNorm(), stream)
   MG_FOR_TYPE(t.dtype, MG_CALL);
 #undef MG_CALL
 }
@@ -652,6 +773,63 @@ hipError_t launch_row_sums(const TokenArg& t, const void* grad, const DropArg& d
 hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
                                  float* grad_scales, hipStream_t stream) {
 #define MG_CALL(T) scale_gradient<T>(t, grad, table, grad_scales, stream)
+  MG_FOR_TYPE(t.dtype, MG_CALL);
+#undef MG_CALL
+}
+
+// encode's backward pass: rows in teams are summed and normed back in one launch; otherwise the sums
+// of all rows go through memory (first in the workspace), and layer_norm.hip takes them back.
+namespace {
+bool sums_in_memory(const TokenArg& t) {
+  return t.ntokens == 0 || t.nrows <= kFewRows || t.channels > kMostTeamChannels;
+}
+struct EncodeLayout {
+  size_t params, rest, bytes;   // offsets: partial sums of weight and bias, workspace of the row sums
+};
+EncodeLayout encode_layout(const TokenArg& t) {
+  EncodeLayout l;
+  l.params = sums_in_memory(t) ? round_up((size_t)t.nrows * t.channels * sizeof(float)) : 0;
+  l.rest = l.params + round_up(sums_in_memory(t)
+                                   ? norm_backward_workspace_bytes(t.nrows, t.channels)
+                                   : (size_t)(t.nrows < kRowParts ? t.nrows : kRowParts) * 2 * t.channels * sizeof(float));
+  l.bytes = l.rest + (t.ntokens ? embed_backward_workspace_bytes(t.ntokens, t.nrows, t.channels) : 0);
+  return l;
+}
+template <typename T>
+hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad, const void* table, float scale,
+                           const DropArg& drop, void* grad_table, void* grad_weight, void* grad_bias,
+                           char* workspace, hipStream_t stream) {
+  const EncodeLayout l = encode_layout(t);
+  const SumArg a{1.f, nullptr, drop};
+  float* params = reinterpret_cast<float*>(workspace + l.params);
+  if (!sums_in_memory(t)) {
+    const TableNorm norm{table, scale, n, grad_table != nullptr, grad_weight || grad_bias,
+                         {params, grad_weight, grad_bias, n.param_dtype == MG_FLOAT32}};
+    return sorted_rows<T, true, true>(t, grad, a, grad_table, workspace + l.rest, norm, stream);
+  }
+  float* sums = reinterpret_cast<float*>(workspace);
+  hipError_t e = t.nrows == 0 ? hipSuccess
+                 : t.ntokens == 0 ? zero<float>(sums, (size_t)t.nrows * t.channels, stream)
+                 : t.nrows <= kFewRows
+                     ? few_rows<T, float, true>(t, grad, a, sums, (float*)(workspace + l.rest), stream)
+                     : wide_rows<T, float, true>(t, grad, a, sums, workspace + l.rest, stream);
+  if (e != hipSuccess) return e;
+  return launch_table_norm_backward(n, sums, table, scale, grad_table, grad_weight, grad_bias, params, stream);
+}
+}  // namespace
+
+size_t encode_backward_workspace_bytes(int ntokens, int nrows, int channels) {
+  TokenArg t{};
+  t.ntokens = ntokens;
+  t.nrows = nrows;
+  t.channels = channels;
+  return encode_layout(t).bytes;
+}
+hipError_t launch_encode_backward(const TokenArg& t, const NormArg& a, const void* grad, const void* table,
+                                  float scale, const DropArg& drop, void* grad_table, void* grad_weight,
+                                  void* grad_bias, void* workspace, hipStream_t stream) {
+#define MG_CALL(T) \
+  encode_backward<T>(t, a, grad, table, scale, drop, grad_table, grad_weight, grad_bias, (char*)workspace, stream)
   MG_FOR_TYPE(t.dtype, MG_CALL);
 #undef MG_CALL
 }

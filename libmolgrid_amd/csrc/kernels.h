@@ -119,15 +119,10 @@ hipError_t launch_interpolate(const InterpArg& p, int nbatch, const Vec3Arg& in_
 // Learned type vectors (embed.hip, layer_norm.hip, dropout.hip)
 hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const float* scales,
                         void* out, hipStream_t stream);
-// The gradient of the table, and the sums of the kept, scaled-up gradients of every row's tokens
-// in float (the first half of launch_encode's backward pass); both need
-// row_sums_workspace_bytes().
-size_t row_sums_workspace_bytes(int ntokens, int nrows, int channels);
+size_t embed_backward_workspace_bytes(int ntokens, int nrows, int channels);
 hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scale,
                                  const float* scales, void* grad_table, void* workspace,
                                  hipStream_t stream);
-hipError_t launch_row_sums(const TokenArg& t, const void* grad, const DropArg& drop, float* out,
-                           void* workspace, hipStream_t stream);
 hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
                                  float* grad_scales, hipStream_t stream);
 
@@ -143,11 +138,20 @@ hipError_t launch_table_norm_backward(const NormArg& a, const float* sums, const
                                       float scale, void* grad_table, void* grad_weight,
                                       void* grad_bias, void* workspace, hipStream_t stream);
 
+// The partial sums of `parts` workgroups (ParamSums), added up.
+hipError_t launch_sum_partials(const NormArg& a, const float* partial, int parts, void* grad_weight,
+                               void* grad_bias, hipStream_t stream);
+
 hipError_t launch_dropout(const void* in, size_t n, int dtype, const DropArg& drop, void* out,
                           hipStream_t stream);
 
 hipError_t launch_encode(const TokenArg& t, const NormArg& a, const void* table, float scale,
                          const void* bias, const DropArg& drop, void* out, hipStream_t stream);
+size_t encode_backward_workspace_bytes(int ntokens, int nrows, int channels);
+hipError_t launch_encode_backward(const TokenArg& t, const NormArg& a, const void* grad,
+                                  const void* table, float scale, const DropArg& drop,
+                                  void* grad_table, void* grad_weight, void* grad_bias,
+                                  void* workspace, hipStream_t stream);
 
 // float <-> double copies (convert.hip)
 hipError_t launch_widen(const float* src, double* dst, size_t n, hipStream_t stream);

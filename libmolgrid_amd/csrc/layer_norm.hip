@@ -63,7 +63,6 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
   float w[K][VEC], b[K][VEC];
   load_param<T, VEC, LANES, K>(a.weight, a.param_dtype == MG_FLOAT32, 1.f, channels, lane, w);
   load_param<T, VEC, LANES, K>(bias, a.param_dtype == MG_FLOAT32, 0.f, channels, lane, b);
-  const float inv = 1.f / channels;
   const uint32_t step = gridDim.x * Shape::TEAMS;
 
   RowPacks<T, VEC, K> next;
@@ -85,28 +84,13 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
     const bool named = next_named;
     fetch(n + step);
     float v[K][VEC];
-    float sum[1] = {0.f}, squares[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[k][i] = widen(packs.pack[k].v[i]);
-        if (ENCODE) v[k][i] *= scale;
-        sum[0] += v[k][i];
-      }
-    team_sums<LANES>(sum, slots[0]);
-    const float mean = sum[0] / channels;   // (a product could be contracted into the differences)
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const bool inside = (k * LANES + lane) * VEC < channels;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[k][i] = inside ? v[k][i] - mean : 0.f;
-        squares[0] = fmaf(v[k][i], v[k][i], squares[0]);
-      }
-    }
-    team_sums<LANES>(squares, slots[1]);
-    const float rstd = 1.f / sqrtf(fmaf(squares[0], inv, a.eps));
+      for (int i = 0; i < VEC; ++i)
+        v[k][i] = ENCODE ? scale * widen(packs.pack[k].v[i]) : widen(packs.pack[k].v[i]);
+    float mean, rstd;
+    team_stats<VEC, LANES, K>(v, channels, lane, a.eps, slots[0], slots[1], mean, rstd);
     if (n >= nrows) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -166,16 +150,15 @@ __global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenAr
 }
 
 // Backward: a team holds the rows of x and of the gradient, writes dx, and a lane adds its share of
-// dw and db up over all rows that its team takes.  At the end the workgroup's teams are added in
-// their order, and the workgroup writes one row of `partial` (dw, then db).  G: type of the
-// gradient; TABLE: x is a scaled table, whose statistics are computed here.
+// dw and db up over all rows that its team takes.  G: type of the gradient; TABLE: x is a scaled
+// table, whose statistics are computed here.
 constexpr int kParts = 512;
 
 template <typename T, typename G, int VEC, int LANES, int K, bool TABLE>
 __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_kernel(
     const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a,
     const float* __restrict__ means, const float* __restrict__ rstds, T* __restrict__ grad_x,
-    float* __restrict__ partial) {
+    bool to_params, ParamSums params) {
   using Shape = TeamShape<LANES, K>;
   __shared__ float slots[4][2 * Shape::WAVES];
   HIP_DYNAMIC_SHARED(float, sums);   // dw and db of a workgroup with several teams
@@ -218,22 +201,8 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[k][i] = TABLE ? scale * widen(px.pack[k].v[i]) : widen(px.pack[k].v[i]);
     if (TABLE) {
-      float sum[1] = {0.f}, squares[1] = {0.f};
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[0] += h[k][i];
-      team_sums<LANES>(sum, slots[2]);
-      mean = sum[0] / channels;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float d = (k * LANES + lane) * VEC < channels ? h[k][i] - mean : 0.f;
-          squares[0] = fmaf(d, d, squares[0]);
-        }
-      team_sums<LANES>(squares, slots[3]);
-      rstd = 1.f / sqrtf(fmaf(squares[0], inv, a.eps));
+      team_stats<VEC, LANES, K>(h, channels, lane, a.eps, slots[2], slots[3], mean, rstd);
+      mean = 0.f;   // (taken out already)
     }
     float both[2] = {0.f, 0.f};
 #pragma unroll
@@ -265,46 +234,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
       store_floats<T, VEC>(grad_x + (size_t)n * channels + c, d);
     }
   }
-  if (partial == nullptr) return;
-
-  // the teams of a wave, then the waves of the workgroup
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-      for (int m = LANES; m < kWave; m *= 2) {
-        dw[k][i] += __shfl_xor(dw[k][i], m);
-        db[k][i] += __shfl_xor(db[k][i], m);
-      }
-    }
-  constexpr int kTurns = LANES < kWave ? Shape::WAVES : Shape::TEAMS;   // one after the other
-  const int turn = LANES < kWave ? threadIdx.x / kWave : team;
-  const bool speaks = LANES >= kWave || (threadIdx.x & (kWave - 1)) < LANES;
-  for (int t = 0; t < kTurns; ++t) {
-    if (t > 0) lds_barrier();
-    if (turn != t || !speaks) continue;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * LANES + lane) * VEC;
-      if (c >= channels) break;
-      float* to_w = partial + (size_t)blockIdx.x * 2 * channels + c;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (t > 0) {
-          dw[k][i] += sums[c + i];
-          db[k][i] += sums[channels + c + i];
-        }
-        if (t + 1 < kTurns) {
-          sums[c + i] = dw[k][i];
-          sums[channels + c + i] = db[k][i];
-        } else {
-          to_w[i] = dw[k][i];
-          to_w[channels + i] = db[k][i];
-        }
-      }
-    }
-  }
+  if (to_params) add_up_params<T, VEC, LANES, K>(dw, db, lane, channels, sums, params);
 }
 
 // The same for rows wider than any team: dx, a workgroup a row, and dw and db, a thread a channel.
@@ -383,11 +313,12 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_partials_kernel(
 int wide_parts(int nrows) { return nrows < 256 ? nrows : 256; }
 
 template <typename P>
-void sum_partials(const float* partial, int parts, int channels, void* grad_weight, void* grad_bias,
+hipError_t sum_partials(const float* partial, int parts, int channels, void* grad_weight, void* grad_bias,
                   hipStream_t stream) {
   hipLaunchKernelGGL((sum_partials_kernel<P>), dim3(((size_t)2 * channels + kWave - 1) / kWave),
                      dim3(kWave * kSumWaves), 0, stream, partial, parts, channels, (P*)grad_weight,
                      (P*)grad_bias);
+  return hipGetLastError();
 }
 
 template <typename T, bool ENCODE>
@@ -429,7 +360,9 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
                          void* grad_bias, void* workspace, hipStream_t stream) {
   const bool to_params = grad_weight || grad_bias;
   float* partial = to_params ? static_cast<float*>(workspace) : nullptr;
+  const ParamSums params{partial, grad_weight, grad_bias, a.param_dtype == MG_FLOAT32};
   int parts = 0;
+  bool done = false;
   if (a.nrows > 0) {
     const auto with_packs = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
@@ -439,12 +372,12 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
         const size_t shared = S::LANES <= kWave ? (size_t)2 * a.channels * sizeof(float) : 0;
         hipLaunchKernelGGL((norm_backward_kernel<T, G, VEC, S::LANES, S::K, TABLE>), dim3(parts),
                            dim3(S::THREADS), shared, stream, (const G*)grad, (const T*)x, scale, a,
-                           means, rstds, (T*)grad_x, partial);
+                           means, rstds, (T*)grad_x, to_params, params);
       });
     };
     const bool whole = whole_packs<T>(a.channels, address(x) | address(grad) | address(grad_x));
-    const bool done = whole ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
-                            : with_packs(std::integral_constant<int, 1>());
+    done = whole ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
+                 : with_packs(std::integral_constant<int, 1>());
     if (!done) {
       parts = wide_parts(a.nrows);
       if (grad_x)
@@ -456,12 +389,8 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
                            (const G*)grad, (const T*)x, scale, a, means, rstds, partial);
     }
   }
-  if (to_params) {
-    if (a.param_dtype == MG_FLOAT32)
-      sum_partials<float>(partial, parts, a.channels, grad_weight, grad_bias, stream);
-    else
-      sum_partials<T>(partial, parts, a.channels, grad_weight, grad_bias, stream);
-  }
+  if (to_params && !(done && parts == 1))
+    return launch_sum_partials(a, partial, parts, grad_weight, grad_bias, stream);
   return hipGetLastError();
 }
 
@@ -479,6 +408,13 @@ size_t norm_backward_workspace_bytes(int nrows, int channels) {
     case MG_BFLOAT16: return FN(Bfloat16);    \
   }                                           \
   return hipErrorInvalidValue
+
+hipError_t launch_sum_partials(const NormArg& a, const float* partial, int parts, void* grad_weight,
+                               void* grad_bias, hipStream_t stream) {
+#define MG_CALL(T) sum_partials<T>(partial, parts, a.channels, grad_weight, grad_bias, stream)
+  MG_FOR_TYPE(a.param_dtype, MG_CALL);
+#undef MG_CALL
+}
 
 hipError_t launch_norm(const NormArg& a, const void* x, const void* bias, void* out, float* means,
                        float* rstds, hipStream_t stream) {

@@ -17,6 +17,8 @@ struct TeamShape {
   static constexpr int WAVES = THREADS / kWave;
 };
 
+constexpr int kMostTeamChannels = 16384;   // of rows that a team can hold
+
 // Calls f with the shape for rows of `packs` packs: the narrowest team that holds them, in which a
 // lane holds up to 32 elements of 16-bit types, 16 of any other.  False: no team is wide enough.
 template <int VEC, typename F>
@@ -41,6 +43,19 @@ bool with_team(int packs, F f) {
     if (packs <= 4096 * 4 / VEC) return f(TeamShape<1024, 16 / VEC>()), true;
   }
   return false;
+}
+
+// The same for sums over scattered rows, whose loads wait for one another: wider teams, so that a
+// lane has as many rows in flight as it can.
+template <int VEC, typename F>
+bool with_sum_team(int packs, F f) {
+  if constexpr (VEC == 1) {
+    if (packs > 64 && packs <= 256) return f(TeamShape<256, 1>()), true;
+    if (packs > 256 && packs <= 1024) return f(TeamShape<256, 4>()), true;
+  } else {
+    if (packs > 64 && packs <= 256) return f(TeamShape<256, 1>()), true;
+  }
+  return with_team<VEC>(packs, f);
 }
 
 // Elements of a pack for rows of `channels` elements in arrays whose addresses are ORed together in
@@ -112,23 +127,136 @@ __device__ __forceinline__ void load_row(const T* row, int channels, int lane, b
 }
 
 // A lane's share of a parameter (float or of type T, or absent)
-template <typename T, int VEC, int LANES, int K>
-__device__ __forceinline__ void load_param(const void* p, bool is_float, float absent, int channels,
-                                           int lane, float (&out)[K][VEC]) {
+template <typename S, int VEC, int LANES, int K>
+__device__ __forceinline__ void load_param_as(const S* p, int channels, int lane, float (&out)[K][VEC]) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * LANES + lane) * VEC;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) out[k][i] = absent;
-    if (p == nullptr || c >= channels) continue;
-    if (is_float) {
-      const float* f = static_cast<const float*>(p) + c;
+    for (int i = 0; i < VEC; ++i) out[k][i] = c < channels ? widen(p[c + i]) : 0.f;
+  }
+}
+template <typename T, int VEC, int LANES, int K>
+__device__ __forceinline__ void load_param(const void* p, bool is_float, float absent, int channels,
+                                           int lane, float (&out)[K][VEC]) {
+  if (p == nullptr) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[k][i] = f[i];
-    } else {
-      const T* t = static_cast<const T*>(p) + c;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[k][i] = widen(t[i]);
+      for (int i = 0; i < VEC; ++i) out[k][i] = absent;
+  } else if (is_float) {
+    load_param_as<float, VEC, LANES, K>(static_cast<const float*>(p), channels, lane, out);
+  } else {
+    load_param_as<T, VEC, LANES, K>(static_cast<const T*>(p), channels, lane, out);
+  }
+}
+
+// The rows of tokens n[0 .. U) below `end`, -1 for the others: all their indices are loaded together.
+template <int U>
+__device__ __forceinline__ void token_rows(const TokenArg& t, const uint32_t (&n)[U], uint32_t end,
+                                           int (&row)[U]) {
+#define MG_ROWS(S)                                                                  \
+  {                                                                                 \
+    S index[U];                                                                     \
+    _Pragma("unroll") for (int u = 0; u < U; ++u)                                   \
+      index[u] = n[u] < end ? static_cast<const S*>(t.index)[n[u]] : (S)-1;         \
+    _Pragma("unroll") for (int u = 0; u < U; ++u) row[u] = table_row(index[u], t.nrows); \
+  }
+  if (t.index_kind == MG_INDEX_FLOAT32)
+    MG_ROWS(float)
+  else if (t.index_kind == MG_INDEX_INT32)
+    MG_ROWS(int32_t)
+  else
+    MG_ROWS(int64_t)
+#undef MG_ROWS
+}
+
+// Statistics of the row that a team holds in v, which becomes its differences from the mean; two
+// slots arrays as in team_sums.
+template <int VEC, int LANES, int K>
+__device__ __forceinline__ void team_stats(float (&v)[K][VEC], int channels, int lane, float eps,
+                                           float* slots_a, float* slots_b, float& mean, float& rstd) {
+  float sum[1] = {0.f}, squares[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[0] += v[k][i];
+  team_sums<LANES>(sum, slots_a);
+  mean = sum[0] / channels;   // (a product could be contracted into the differences)
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool inside = (k * LANES + lane) * VEC < channels;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      v[k][i] = inside ? v[k][i] - mean : 0.f;
+      squares[0] = fmaf(v[k][i], v[k][i], squares[0]);
+    }
+  }
+  team_sums<LANES>(squares, slots_b);
+  rstd = 1.f / sqrtf(squares[0] / channels + eps);
+}
+
+// Where the sums of a norm's parameter gradients go: as they are if one workgroup has them all,
+// else into the workgroup's row of `partial` (weight, then bias).
+struct ParamSums {
+  float* partial;
+  void *weight, *bias;   // of param_dtype; either may be nullptr
+  int is_float;
+};
+template <typename T>
+__device__ __forceinline__ void store_param_sum(const ParamSums& to, int channels, int c, float dw, float db) {
+  if (gridDim.x > 1) {
+    float* row = to.partial + (size_t)blockIdx.x * 2 * channels;
+    row[c] = dw;
+    row[channels + c] = db;
+  } else if (to.is_float) {
+    if (to.weight) static_cast<float*>(to.weight)[c] = dw;
+    if (to.bias) static_cast<float*>(to.bias)[c] = db;
+  } else {
+    if (to.weight) static_cast<T*>(to.weight)[c] = narrow<T>(dw);
+    if (to.bias) static_cast<T*>(to.bias)[c] = narrow<T>(db);
+  }
+}
+
+// Adds the teams' shares of dw and db up in their order: those of a wave first, then the waves one
+// after the other through `sums` (2 channels floats of LDS, where a workgroup has several teams).
+template <typename T, int VEC, int LANES, int K>
+__device__ __forceinline__ void add_up_params(float (&dw)[K][VEC], float (&db)[K][VEC], int lane, int channels,
+                                              float* sums, const ParamSums& to) {
+  using Shape = TeamShape<LANES, K>;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+      for (int m = LANES; m < kWave; m *= 2) {
+        dw[k][i] += __shfl_xor(dw[k][i], m);
+        db[k][i] += __shfl_xor(db[k][i], m);
+      }
+    }
+  constexpr int kTurns = LANES < kWave ? Shape::WAVES : Shape::TEAMS;
+  const int turn = LANES < kWave ? threadIdx.x / kWave : threadIdx.x / LANES;
+  const bool speaks = LANES >= kWave || (threadIdx.x & (kWave - 1)) < LANES;
+  for (int t = 0; t < kTurns; ++t) {
+    if (t > 0) lds_barrier();
+    if (turn != t || !speaks) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c >= channels) break;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (t > 0) {
+          dw[k][i] += sums[c + i];
+          db[k][i] += sums[channels + c + i];
+        }
+        if (t + 1 < kTurns) {
+          sums[c + i] = dw[k][i];
+          sums[channels + c + i] = db[k][i];
+        } else {
+          store_param_sum<T>(to, channels, c + i, dw[k][i], db[k][i]);
+        }
+      }
     }
   }
 }

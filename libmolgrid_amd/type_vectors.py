@@ -20,6 +20,7 @@ tensors.  Type indices are float32 (as coordinate sets keep them: the whole numb
 int32 or int64 of any shape; an index that names no row gives a row of zeros and no gradient.
 Everything runs on torch's current stream, nothing synchronises.
 """
+import functools
 import math
 
 import numpy as np
@@ -45,7 +46,11 @@ def _is_array(x):
 def _staged(fn):
     """Grid views and managed grids stand for their tensors; where every array is a host array the
     call runs on copies on the device and its tensors come back to the host."""
+    @functools.wraps(fn)
     def wrapper(*args, **kw):
+        first = args[0] if args else None
+        if isinstance(first, torch.Tensor) and first.is_cuda:
+            return fn(*args, **kw)
         args = [_gr._unwrap(a) for a in args]
         kw = {k: _gr._unwrap(v) for k, v in kw.items()}
         arrays = [a for a in list(args) + list(kw.values()) if _is_array(a)]
@@ -60,7 +65,6 @@ def _staged(fn):
                 return tuple(back(x) for x in r)
             return r.cpu() if isinstance(r, torch.Tensor) else r
         return back(fn(*[there(a) for a in args], **{k: there(v) for k, v in kw.items()}))
-    wrapper.__name__, wrapper.__doc__ = fn.__name__, fn.__doc__
     return wrapper
 
 
@@ -68,7 +72,9 @@ def _tensor(x, name, dtypes):
     """The checks of gridding's device arrays (python/bindings_grids.cpp:91-137): a contiguous
     tensor of a supported type on the current device."""
     if not isinstance(x, torch.Tensor):
-        raise ValueError("%s: expected a tensor" % name)
+        x = _gr._unwrap(x)
+        if not isinstance(x, torch.Tensor):
+            raise ValueError("%s: expected a tensor" % name)
     if x.dtype not in dtypes:
         raise ValueError("%s: %s is not supported here" % (name, x.dtype))
     if not x.is_cuda:
