@@ -90,10 +90,10 @@ __device__ __forceinline__ int table_row(float index, int nrows) {
   return row < nrows ? row : -1;
 }
 __device__ __forceinline__ int table_row(int32_t index, int nrows) {
-  return index >= 0 && index < nrows ? index : -1;
+  return (uint32_t)index < (uint32_t)nrows ? index : -1;
 }
 __device__ __forceinline__ int table_row(int64_t index, int nrows) {
-  return index >= 0 && index < (int64_t)nrows ? (int)index : -1;
+  return (uint64_t)index < (uint64_t)nrows ? (int)index : -1;
 }
 
 __device__ __forceinline__ int token_row(const TokenArg& t, size_t n) {
@@ -123,7 +123,7 @@ __device__ __forceinline__ Words4 philox(uint64_t low, uint64_t high, uint64_t k
 #pragma unroll
   for (int round = 0; round < 10; ++round) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    const uint32_t n0 = (uint32_t)(b >> 32) ^ c1 ^ k0, n2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    const uint32_t n0 = xor3((uint32_t)(b >> 32), c1, k0), n2 = xor3((uint32_t)(a >> 32), c3, k1);
     c1 = (uint32_t)b;
     c3 = (uint32_t)a;
     c0 = n0;

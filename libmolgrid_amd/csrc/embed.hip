@@ -43,15 +43,12 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(TokenArg t, const T* __
     }
     for (int c0 = lane * VEC; c0 < t.channels; c0 += LANES * VEC * kUnroll) {
       float v[kUnroll][VEC];
+      if (t.nrows > 0)
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int c = c0 + u * LANES * VEC;
-        if (at >= 0 && c < t.channels)
-          load_floats<T, VEC>(from + c, v[u]);
-        else
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[u][i] = 0.f;
-      }
+        for (int u = 0; u < kUnroll; ++u) {   // (beyond the last channel: the first ones, not used)
+          const int c = c0 + u * LANES * VEC;
+          load_floats<T, VEC>(from + (c < t.channels ? c : 0), v[u]);
+        }
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int c = c0 + u * LANES * VEC;
@@ -204,15 +201,15 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kSortRange = 960;   // most rows of a workgroup: 60 KB of counters
 
 // A row of up to kDirect tokens is added up by one team.  Longer ones are cut into pieces that
-// start at multiples of their length from the row's start: about as many pieces as a piece has
-// tokens, a multiple of kBlock.  A piece's sum has slot 2 b + f, where b is the block of kBlock
+// start at multiples of their length from the row's start, a multiple of kBlock tokens, so that the
+// tokens of a piece and the pieces of a row, which are added up one after the other, stay balanced.  A piece's sum has slot 2 b + f, where b is the block of kBlock
 // positions of the order that the piece starts in and f whether it is its row's first: of a block's
 // positions at most two start pieces, a first one (its row then holds the block's last position) and
 // a later one (its row then holds the block's first position).
-constexpr int kBlock = 32, kDirect = 64;
+constexpr int kBlock = 16, kDirect = 32;
 
 __device__ __forceinline__ int piece_length(int count) {
-  return ((int)sqrtf((float)count) / kBlock + 1) * kBlock;
+  return ((int)(0.5f * sqrtf((float)count)) / kBlock + 1) * kBlock;
 }
 __device__ __forceinline__ int piece_slot(int from, int length, int j) {
   return (from + j * length) / kBlock * 2 + (j == 0 ? 1 : 0);
@@ -253,17 +250,18 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
   int lower = 0;
   uint64_t held = 0;   // bit b of lane l: step 64 l + b has a token of this workgroup's rows
   for (uint32_t s0 = 0; s0 < steps; s0 += kAhead) {
-    int row[kAhead];
+    uint32_t row[kAhead];   // (no row: larger than any)
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) row[u] = fetch(begin + (s0 + u) * kWave + lane);
+    for (int u = 0; u < kAhead; ++u) row[u] = (uint32_t)fetch(begin + (s0 + u) * kWave + lane);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      lower += row[u] >= 0 && row[u] < row0 ? 1 : 0;
-      const int r = row[u] - row0;
-      const bool inside = row[u] >= row0 && r < rows;
-      if (inside) atomicAdd(&mine[r], 1);
-      const uint32_t s = s0 + u;
-      if (__ballot(inside) && (uint32_t)lane == s / 64) held |= (uint64_t)1 << (s % 64);
+      lower += row[u] < (uint32_t)row0 ? 1 : 0;
+      const uint32_t r = row[u] - (uint32_t)row0, s = s0 + u;
+      const bool inside = r < (uint32_t)rows;
+      if (__ballot(inside)) {
+        if (inside) atomicAdd(&mine[r], 1);
+        if ((uint32_t)lane == s / 64) held |= (uint64_t)1 << (s % 64);
+      }
     }
   }
   lower = wave_inclusive_sum(lower, lane);
@@ -293,26 +291,40 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
     if (row0 + r == nrows - 1) sorted.start[nrows] = at;
   }
   __syncthreads();
-  // slots of the blocks of the order that this workgroup's rows hold the first or last position of
-  if (sorted.piece_row)
-    for (int i = wave; i < rows; i += kSortWaves) {
+  // Slots of the blocks of the order that this workgroup's rows hold the first or last position of:
+  // a thread does those of its row, a wave those of a row that is cut.
+  if (sorted.piece_row) {
+    for (int i = threadIdx.x; i < rows; i += kSortThreads) {
       const int from = count[i], to = i + 1 < rows ? count[i + 1] : last;
-      const bool cut = to - from > kDirect;
-      const int length = piece_length(to - from);
-      for (int b = from / kBlock + lane; b * kBlock < to; b += kWave) {
-        const int first = b * kBlock;
-        if (first >= from) {
-          const int j = (first - from + length - 1) / length, p = from + j * length;
-          sorted.piece_row[2 * b] = cut && j > 0 && p < to && p < first + kBlock ? row0 + i : -1;
-        }
-        if (first + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = cut && first <= from ? row0 + i : -1;
+      if (to - from > kDirect) continue;
+      for (int b = from / kBlock; b * kBlock < to; ++b) {
+        if (b * kBlock >= from) sorted.piece_row[2 * b] = -1;
+        if (b * kBlock + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = -1;
       }
     }
+    for (int i0 = wave * kWave; i0 < rows; i0 += kSortWaves * kWave) {
+      const int i1 = i0 + lane, end_of = i1 + 1 < rows ? count[min(i1 + 1, rows - 1)] : last;
+      unsigned long long cut = __ballot(i1 < rows && end_of - count[min(i1, rows - 1)] > kDirect);
+      for (; cut; cut &= cut - 1) {
+        const int i = i0 + (int)__builtin_ctzll(cut);
+        const int from = count[i], to = i + 1 < rows ? count[i + 1] : last;
+        const int length = piece_length(to - from);
+        for (int b = from / kBlock + lane; b * kBlock < to; b += kWave) {
+          const int first = b * kBlock;
+          if (first >= from) {
+            const int j = (first - from + length - 1) / length, p = from + j * length;
+            sorted.piece_row[2 * b] = j > 0 && p < to && p < first + kBlock ? row0 + i : -1;
+          }
+          if (first + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = first <= from ? row0 + i : -1;
+        }
+      }
+    }
+  }
   __syncthreads();
   const unsigned long long below = (1ull << lane) - 1;
   const auto place = [&](uint32_t n, int row) {
     const int r = row - row0;
-    const bool inside = row >= row0 && r < rows;
+    const bool inside = row >= 0 && (uint32_t)r < (uint32_t)rows;
     unsigned long long left = __ballot(inside);
     while (left) {   // one turn for each row among the wave's tokens
       const int first = __builtin_amdgcn_readlane(r, (int)__builtin_ctzll(left));
@@ -355,33 +367,44 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
   }
 }
 
-// Adds the tokens order[begin .. end) to acc, in that order.
+// Tokens of a team in flight, and the first ones of order[begin .. end)
+constexpr int tokens_ahead(int packs) { return packs == 1 ? 8 : 4; }
+template <int U>
+__device__ __forceinline__ void first_tokens(const int32_t* order, int begin, int end, uint32_t (&n)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (begin + u < end) n[u] = (uint32_t)order[begin + u];
+}
+
+// Adds channels c0 + ... of the tokens order[begin .. end) to acc, in that order; `n` are the first of
+// them.  The next ones are read while the gradients of these are under way.
 template <typename T, int VEC, int LANES, int K, bool DROP>
 __device__ __forceinline__ void add_tokens(const TokenArg& t, const T* grad, const SumArg& a,
-                                           const int32_t* order, int begin, int end, int lane,
-                                           uint64_t seed, uint64_t offset, float (&acc)[K][VEC]) {
-  constexpr int kAhead = K == 1 ? 8 : K <= 4 ? 4 : 2;
-  for (int i0 = begin; i0 < end; i0 += kAhead) {
-    RowPacks<T, VEC, K> g[kAhead];
-    uint32_t n[kAhead];
-    float by[kAhead];
+                                           const int32_t* order, int begin, int end, int c0, int lane,
+                                           uint64_t seed, uint64_t offset,
+                                           uint32_t (&n)[tokens_ahead(K)], float (&acc)[K][VEC]) {
+  constexpr int U = tokens_ahead(K);
+  for (int i0 = begin; i0 < end; i0 += U) {
+    RowPacks<T, VEC, K> g[U];
+    uint32_t now[U];
+    float by[U];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) n[u] = i0 + u < end ? (uint32_t)order[i0 + u] : 0;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const bool live = i0 + u < end;
-      by[u] = !live ? 0.f : a.scales ? a.scales[n[u]] : a.scale;
-      load_row<T, VEC, LANES, K>(grad + (size_t)n[u] * t.channels, t.channels, lane, live, g[u]);
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= end) break;
+      now[u] = n[u];
+      by[u] = a.scales ? a.scales[n[u]] : a.scale;
+      load_row<T, VEC, LANES, K>(grad + (size_t)n[u] * t.channels + c0, t.channels - c0, lane, true, g[u]);
     }
+    first_tokens(order, i0 + U, end, n);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (i0 + u >= end) break;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float v[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = widen(g[u].pack[k].v[i]);
-        add_token<DROP, VEC>((size_t)n[u] * t.channels + (k * LANES + lane) * VEC, a, by[u], seed, offset, v,
+        add_token<DROP, VEC>((size_t)now[u] * t.channels + c0 + (k * LANES + lane) * VEC, a, by[u], seed, offset, v,
                              acc[k]);
       }
     }
@@ -397,13 +420,14 @@ __device__ __forceinline__ void store_row(O* to, int channels, int lane, const f
   }
 }
 
-// The pieces of long rows, a team a slot.
+// The pieces of long rows, a team a slot; tiles of channels along the grid's y.
 template <typename T, int VEC, int LANES, int K, bool DROP>
-__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void pieces_kernel(
-    TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted, float* __restrict__ partial) {
+__global__ __launch_bounds__(kThreads) void pieces_kernel(TokenArg t, const T* __restrict__ grad,
+                                                          SumArg a, Sorted sorted,
+                                                          float* __restrict__ partial) {
   const int lane = threadIdx.x % LANES;
-  const int slot = blockIdx.x * TeamShape<LANES, K>::TEAMS + threadIdx.x / LANES;
-  const int block = slot / 2;
+  const int slot = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int block = slot / 2, c0 = blockIdx.y * LANES * K * VEC;
   if ((int64_t)block * kBlock + (slot & 1 ? kBlock - 1 : 0) >= sorted.start[t.nrows]) return;
   const int row = sorted.piece_row[slot];
   if (row < 0) return;
@@ -413,8 +437,10 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void pieces_kernel(
   const int j = slot & 1 ? 0 : (block * kBlock - from + length - 1) / length;
   const int begin = from + j * length, end = min(begin + length, to);
   float acc[K][VEC] = {};
-  add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, begin, end, lane, seed, offset, acc);
-  store_row<float, VEC, LANES, K>(partial + (size_t)slot * t.channels, t.channels, lane, acc);
+  uint32_t n[tokens_ahead(K)];
+  first_tokens(sorted.order, begin, end, n);
+  add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, begin, end, c0, lane, seed, offset, n, acc);
+  store_row<float, VEC, LANES, K>(partial + (size_t)slot * t.channels + c0, t.channels - c0, lane, acc);
 }
 
 // What a row's sum goes through when the vectors were normed rows of the scaled table
@@ -426,19 +452,20 @@ struct TableNorm {
   ParamSums params;
 };
 
-// Every row of the table: the sum of its tokens, or of its pieces.  The bounds of a team's next row
-// are read ahead.  NORM: the sum is the gradient of the row's normed vector, which is taken back
-// through the norm while it is here; the workgroups then stay, and their teams' shares of the
-// gradients of weight and bias are added up at the end.
-template <typename T, int VEC, int LANES, int K, bool DROP, bool NORM>
+// Every row of the table: the sum of its tokens, or of its pieces; tiles of channels along the
+// grid's y.  What the next rows need is read ahead: their bounds two rows, their first tokens one.
+// NORM: the sum is the gradient of the row's normed vector, which is taken back through the norm
+// while it is here (a team then holds the whole row); the workgroups stay, and their teams' shares
+// of the gradients of weight and bias are added up at the end.
+template <typename T, typename O, int VEC, int LANES, int K, bool DROP, bool NORM>
 __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
     TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted,
-    const float* __restrict__ partial, T* __restrict__ out, TableNorm norm) {
+    const float* __restrict__ partial, O* __restrict__ out, TableNorm norm) {
   using Shape = TeamShape<LANES, K>;
   __shared__ float slots[3][2 * Shape::WAVES];
   HIP_DYNAMIC_SHARED(float, param_sums);
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
-  const int channels = t.channels;
+  const int c0 = NORM ? 0 : blockIdx.y * LANES * K * VEC, channels = t.channels - c0;
   const uint32_t nrows = (uint32_t)t.nrows, step = gridDim.x * Shape::TEAMS;
   uint64_t seed = 0, offset = 0;
   if (DROP) drop_key(a.drop, seed, offset);
@@ -450,38 +477,52 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
 #pragma unroll
       for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.f;
   }
+  constexpr int U = tokens_ahead(K);
+  const auto bounds = [&](uint32_t row, int& from, int& to) {
+    from = row < nrows ? sorted.start[row] : 0;
+    to = row < nrows ? sorted.start[row + 1] : 0;
+  };
+  int from1, to1, from2, to2;   // of the next row and the one after it
+  uint32_t n1[U];
   const uint32_t mine = blockIdx.x * Shape::TEAMS + team;
-  int next_from = mine < nrows ? sorted.start[mine] : 0, next_to = mine < nrows ? sorted.start[mine + 1] : 0;
+  bounds(mine, from1, to1);
+  bounds(mine + step, from2, to2);
+  first_tokens(sorted.order, from1, to1, n1);
   for (uint32_t row0 = blockIdx.x * Shape::TEAMS; row0 < nrows; row0 += step) {
     const uint32_t row = row0 + team;
-    const int from = next_from, to = next_to;
-    const bool more = row + step < nrows;
-    next_from = more ? sorted.start[row + step] : 0;
-    next_to = more ? sorted.start[row + step + 1] : 0;
+    const int from = from1, to = to1;
+    uint32_t n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) n[u] = n1[u];
+    from1 = from2;
+    to1 = to2;
+    first_tokens(sorted.order, from1, to1, n1);
+    bounds(row + 2 * step, from2, to2);
     const bool some = to > from;
     float v[K][VEC] = {};
     RowPacks<T, VEC, K> x;
-    if (NORM)
-      load_row<T, VEC, LANES, K>(static_cast<const T*>(norm.table) + (some ? (size_t)row * channels : 0),
-                                 channels, lane, some, x);
+    if (NORM && some)
+      load_row<T, VEC, LANES, K>(static_cast<const T*>(norm.table) + (size_t)row * channels, channels, lane, true, x);
     if (to - from <= kDirect) {
-      add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, from, to, lane, seed, offset, v);
+      add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, from, to, c0, lane, seed, offset, n, v);
     } else {
       const int length = piece_length(to - from), pieces = (to - from + length - 1) / length;
-      constexpr int kAhead = K == 1 ? 8 : K <= 4 ? 4 : 2;
-      for (int j0 = 0; j0 < pieces; j0 += kAhead) {
-        RowPacks<float, VEC, K> p[kAhead];
+      for (int j0 = 0; j0 < pieces; j0 += U) {
+        RowPacks<float, VEC, K> p[U];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          load_row<float, VEC, LANES, K>(
-              partial + (j0 + u < pieces ? (size_t)piece_slot(from, length, j0 + u) * channels : 0), channels,
-              lane, j0 + u < pieces, p[u]);
+        for (int u = 0; u < U; ++u) {
+          if (j0 + u >= pieces) break;
+          load_row<float, VEC, LANES, K>(partial + (size_t)piece_slot(from, length, j0 + u) * t.channels + c0,
+                                         channels, lane, true, p[u]);
+        }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
+        for (int u = 0; u < U; ++u) {
+          if (j0 + u >= pieces) break;
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[k][i] += p[u].pack[k].v[i];
+        }
       }
     }
     // (all teams of a wave come along, and a team of several waves is a workgroup)
@@ -490,7 +531,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) h[k][i] = norm.scale * widen(x.pack[k].v[i]);
+        for (int i = 0; i < VEC; ++i) h[k][i] = some ? norm.scale * widen(x.pack[k].v[i]) : 0.f;
       float mean, rstd;
       team_stats<VEC, LANES, K>(h, channels, lane, norm.norm.eps, slots[0], slots[1], mean, rstd);
       float both[2] = {0.f, 0.f};
@@ -514,30 +555,9 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
           v[k][i] = some ? norm.scale * rstd * (v[k][i] * w[k][i] - mean_q - h[k][i] * mean_qh) : 0.f;
     }
     if (row < nrows && (!NORM || norm.to_table))
-      store_row<T, VEC, LANES, K>(out + (size_t)row * channels, channels, lane, v);
+      store_row<O, VEC, LANES, K>(out + (size_t)row * t.channels + c0, channels, lane, v);
   }
   if (NORM && norm.to_params) add_up_params<T, VEC, LANES, K>(dw, db, lane, channels, param_sums, norm.params);
-}
-
-// Rows wider than any team: a workgroup a row, a thread a channel.
-template <typename T, typename O, bool DROP>
-__global__ __launch_bounds__(kThreads) void wide_rows_kernel(TokenArg t, const T* __restrict__ grad,
-                                                             SumArg a, Sorted sorted,
-                                                             O* __restrict__ out) {
-  uint64_t seed = 0, offset = 0;
-  if (DROP) drop_key(a.drop, seed, offset);
-  for (uint32_t row = blockIdx.x; row < (uint32_t)t.nrows; row += gridDim.x) {
-    const int from = sorted.start[row], to = sorted.start[row + 1];
-    for (int c = blockIdx.y * kThreads + threadIdx.x; c < t.channels; c += gridDim.y * kThreads) {
-      float acc[1] = {0.f};
-      for (int i = from; i < to; ++i) {
-        const uint32_t n = (uint32_t)sorted.order[i];
-        float g[1] = {widen(grad[(size_t)n * t.channels + c])};
-        add_token<DROP, 1>((size_t)n * t.channels + c, a, a.scales ? a.scales[n] : a.scale, seed, offset, g, acc);
-      }
-      out[(size_t)row * t.channels + c] = narrow<O>(acc[0]);
-    }
-  }
 }
 
 // ---- launches -------------------------------------------------------------------------------------
@@ -631,7 +651,7 @@ SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   l.order = round_up(((size_t)nrows + 1) * sizeof(int32_t));
   l.piece_row = l.order + round_up((size_t)ntokens * sizeof(int32_t));
   l.partial = l.piece_row + round_up((size_t)l.slots * sizeof(int32_t));
-  l.bytes = l.partial + (channels <= kMostTeamChannels ? round_up((size_t)l.slots * channels * sizeof(float)) : 0);
+  l.bytes = l.partial + round_up((size_t)l.slots * channels * sizeof(float));
   return l;
 }
 
@@ -678,45 +698,45 @@ void sort_tokens(const TokenArg& t, const Sorted& sorted, hipStream_t stream) {
 constexpr int kRowParts = 1024;
 
 // The sums by row of a table of more than kFewRows rows, or (NORM) what follows from them.
-template <typename T, bool DROP, bool NORM>
+template <typename T, typename O, bool DROP, bool NORM>
 hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, void* out, void* workspace,
-                       TableNorm norm, hipStream_t stream) {
+                       const TableNorm& norm, hipStream_t stream) {
   const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
   char* base = static_cast<char*>(workspace);
   float* partial = reinterpret_cast<float*>(base + l.partial);
-  Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order),
-                l.slots ? reinterpret_cast<int32_t*>(base + l.piece_row) : nullptr};
+  const Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order),
+                      l.slots ? reinterpret_cast<int32_t*>(base + l.piece_row) : nullptr};
   sort_tokens(t, sorted, stream);
   int parts = 0;
   with_packs_of<T>(t.channels, address(grad) | address(out) | address(NORM ? norm.table : nullptr), [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
-    with_sum_team<VEC>((t.channels + VEC - 1) / VEC, [&](auto shape) {
+    const int packs = (t.channels + VEC - 1) / VEC;
+    const auto tiles = [&](auto shape) {
       using S = decltype(shape);
-      if (l.slots)
+      return (unsigned)((packs + S::LANES * S::K - 1) / (S::LANES * S::K));
+    };
+    if (l.slots)
+      with_tile<VEC, VEC == 1 ? 4 : 1>(packs, [&](auto shape) {
+        using S = decltype(shape);
         hipLaunchKernelGGL((pieces_kernel<T, VEC, S::LANES, S::K, DROP>),
-                           dim3((l.slots + S::TEAMS - 1) / S::TEAMS), dim3(S::THREADS), 0, stream, t,
+                           dim3((l.slots + S::TEAMS - 1) / S::TEAMS, tiles(shape)), dim3(kThreads), 0, stream, t,
                            (const T*)grad, a, sorted, partial);
-      parts = (int)at_most(((size_t)t.nrows + S::TEAMS - 1) / S::TEAMS, NORM ? kRowParts : 16384);
+      });
+    const auto rows = [&](auto shape, size_t most, unsigned y) {
+      using S = decltype(shape);
+      parts = (int)at_most(((size_t)t.nrows + S::TEAMS - 1) / S::TEAMS, most);
       const size_t shared = NORM && S::LANES <= kWave ? (size_t)2 * t.channels * sizeof(float) : 0;
-      hipLaunchKernelGGL((rows_kernel<T, VEC, S::LANES, S::K, DROP, NORM>), dim3(parts), dim3(S::THREADS),
-                         shared, stream, t, (const T*)grad, a, sorted, partial, (T*)out, norm);
-    });
+      hipLaunchKernelGGL((rows_kernel<T, O, VEC, S::LANES, S::K, DROP, NORM>), dim3(parts, y), dim3(S::THREADS),
+                         shared, stream, t, (const T*)grad, a, sorted, partial, (O*)out, norm);
+    };
+    if constexpr (NORM)
+      with_sum_team<VEC>(packs, [&](auto shape) { rows(shape, kRowParts, 1); });
+    else
+      with_tile<VEC, 4>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
   });
   if (NORM && norm.to_params && parts > 1)
     return launch_sum_partials(norm.norm, norm.params.partial, parts, norm.params.weight, norm.params.bias,
                                stream);
-  return hipGetLastError();
-}
-
-template <typename T, typename O, bool DROP>
-hipError_t wide_rows(const TokenArg& t, const void* grad, const SumArg& a, void* out, void* workspace,
-                     hipStream_t stream) {
-  const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
-  char* base = static_cast<char*>(workspace);
-  const Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order), nullptr};
-  sort_tokens(t, sorted, stream);
-  hipLaunchKernelGGL((wide_rows_kernel<T, O, DROP>), dim3(at_most(t.nrows, 8192), 16), dim3(kThreads), 0, stream,
-                     t, (const T*)grad, a, sorted, (O*)out);
   return hipGetLastError();
 }
 
@@ -743,7 +763,6 @@ hipError_t zero(void* out, size_t n, hipStream_t stream) {
   }                                           \
   return hipErrorInvalidValue
 
-// A table's gradient has few rows, or rows that are too wide for a team, or is sorted.
 size_t embed_backward_workspace_bytes(int ntokens, int nrows, int channels) {
   if (nrows <= kFewRows) return few_rows_bytes(ntokens, nrows, channels);
   return sorted_layout(ntokens, nrows, channels).bytes;
@@ -760,12 +779,11 @@ hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scal
                                  const float* scales, void* grad_table, void* workspace,
                                  hipStream_t stream) {
   const SumArg a{scale, scales, DropArg()};
-#define MG_CALL(T)                                                                                  \
-  t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)                        \
-  : t.nrows <= kFewRows ? few_rows<T, T, false>(t, grad, a, grad_table, (float*)workspace, stream)  \
-  : t.channels > kMostTeamChannels ? wide_rows<T, T, false>(t, grad, a, grad_table, workspace, stream) \
-                                   : sorted_rows<T, false, false>(t, grad, a, grad_table, workspace, \
-                                                                  TableNorm(), stream)
+#define MG_CALL(T)                                                                                 \
+  t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)                       \
+  : t.nrows <= kFewRows                                                                            \
+      ? few_rows<T, T, false>(t, grad, a, grad_table, (float*)workspace, stream)                   \
+      : sorted_rows<T, T, false, false>(t, grad, a, grad_table, workspace, TableNorm(), stream)
   MG_FOR_TYPE(t.dtype, MG_CALL);
 #undef MG_CALL
 }
@@ -805,14 +823,14 @@ hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad
   if (!sums_in_memory(t)) {
     const TableNorm norm{table, scale, n, grad_table != nullptr, grad_weight || grad_bias,
                          {params, grad_weight, grad_bias, n.param_dtype == MG_FLOAT32}};
-    return sorted_rows<T, true, true>(t, grad, a, grad_table, workspace + l.rest, norm, stream);
+    return sorted_rows<T, T, true, true>(t, grad, a, grad_table, workspace + l.rest, norm, stream);
   }
   float* sums = reinterpret_cast<float*>(workspace);
   hipError_t e = t.nrows == 0 ? hipSuccess
                  : t.ntokens == 0 ? zero<float>(sums, (size_t)t.nrows * t.channels, stream)
                  : t.nrows <= kFewRows
                      ? few_rows<T, float, true>(t, grad, a, sums, (float*)(workspace + l.rest), stream)
-                     : wide_rows<T, float, true>(t, grad, a, sums, workspace + l.rest, stream);
+                     : sorted_rows<T, float, true, false>(t, grad, a, sums, workspace + l.rest, TableNorm(), stream);
   if (e != hipSuccess) return e;
   return launch_table_norm_backward(n, sums, table, scale, grad_table, grad_weight, grad_bias, params, stream);
 }

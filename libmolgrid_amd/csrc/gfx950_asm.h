@@ -39,6 +39,11 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 // moving LDS accesses across the point.
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_wave_barrier(); }
 
+// a ^ b ^ c
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 // Bits of a 16-bit float type from a float (to the nearest, ties to even) and back.
 __device__ __forceinline__ float half_bits_to_float(uint16_t bits) {
   return (float)__builtin_bit_cast(_Float16, bits);

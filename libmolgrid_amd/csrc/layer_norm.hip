@@ -63,6 +63,16 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
   float w[K][VEC], b[K][VEC];
   load_param<T, VEC, LANES, K>(a.weight, a.param_dtype == MG_FLOAT32, 1.f, channels, lane, w);
   load_param<T, VEC, LANES, K>(bias, a.param_dtype == MG_FLOAT32, 0.f, channels, lane, b);
+  if (ENCODE) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        w[k][i] *= arg.factor;
+        b[k][i] *= arg.factor;
+      }
+    arg.factor = 1.f;
+  }
   const uint32_t step = gridDim.x * Shape::TEAMS;
 
   RowPacks<T, VEC, K> next;
@@ -70,10 +80,12 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
   const auto fetch = [&](uint32_t n) {
     size_t at = n;
     bool live = n < nrows;
+    if (!live) at = 0;
     if (ENCODE) {
       const int row = live ? token_row(tokens, n) : -1;
       at = row < 0 ? 0 : row;
       live = next_named = row >= 0;
+      if (a.nrows == 0) return;
     }
     load_row<T, VEC, LANES, K>(x + at * channels, channels, lane, live, next);
   };

@@ -58,6 +58,18 @@ bool with_sum_team(int packs, F f) {
   return with_team<VEC>(packs, f);
 }
 
+// Teams of a wave or less for rows that are gone through in tiles of up to `most` packs a lane
+template <int VEC, int MOST, typename F>
+void with_tile(int packs, F f) {
+  if (VEC > 1 && packs <= 4) return f(TeamShape<4, 1>());
+  if (VEC > 1 && packs <= 8) return f(TeamShape<8, 1>());
+  if (packs <= 16) return f(TeamShape<16, 1>());
+  if (VEC > 1 && packs <= 32) return f(TeamShape<32, 1>());
+  if (packs <= 64 || MOST == 1) return f(TeamShape<64, 1>());
+  if (packs <= 128 || MOST == 2) return f(TeamShape<64, 2>());
+  return f(TeamShape<64, 4>());
+}
+
 // Elements of a pack for rows of `channels` elements in arrays whose addresses are ORed together in
 // `where`: 16 bytes where every row of every array starts on a 16-byte boundary, one element
 // otherwise.
@@ -112,18 +124,21 @@ template <typename T, int VEC, int K>
 struct RowPacks {
   Pack<T, VEC> pack[K];
 };
+// Lanes beyond the last channel read the row's first pack, which is there, and get zeros: a branch
+// around every load would be issued one after the other.
 template <typename T, int VEC, int LANES, int K>
 __device__ __forceinline__ void load_row(const T* row, int channels, int lane, bool live,
                                          RowPacks<T, VEC, K>& out) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * LANES + lane) * VEC;
-    if (live && c < channels)
-      out.pack[k] = *reinterpret_cast<const Pack<T, VEC>*>(row + c);
-    else
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out.pack[k].v[i] = T();
+    out.pack[k] = *reinterpret_cast<const Pack<T, VEC>*>(row + (c < channels ? c : 0));
   }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (!(live && (k * LANES + lane) * VEC < channels)) out.pack[k].v[i] = T();
 }
 
 // A lane's share of a parameter (float or of type T, or absent)

@@ -92,13 +92,13 @@ def _ptr(x):
 
 
 def _empty(shape, like, dtype=None):
-    return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+    return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
 
 
 def _workspace(size, like):
     """Device memory of one call: the allocator hands it to later work of this stream only, and a
     captured graph's calls get theirs from that graph's pool."""
-    return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
+    return like.new_empty(size, dtype=torch.uint8) if size else None
 
 
 def _count(n, name):
@@ -191,7 +191,7 @@ def embed_types_backward(grad, type_index, table, scale=1.0, table_gradient=True
     index, table, (n, rows, channels) = _table_args(type_index, table)
     number, scales = _scale_args(scale, index)
     grad = _like(grad, "grad", tuple(index.shape) + (channels,), table.dtype)
-    to_table = _empty(table.shape, table) if table_gradient else None
+    to_table = torch.empty_like(table) if table_gradient else None
     to_scale = _empty(index.shape, table, torch.float32) if scale_gradient and scales is not None \
         else None
     size = _capi.lib.mg_embed_types_backward_workspace_size(n, rows, channels) if table_gradient else 0
@@ -219,8 +219,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     weight = _param(weight, "weight", channels, x.dtype)
     bias = _param(bias, "bias", channels, x.dtype, weight)
     params = weight if weight is not None else bias
-    out = _empty(x.shape, x)
-    mean, rstd = (_empty(x.shape[:-1], x, torch.float32) for _ in range(2))
+    out = torch.empty_like(x)
+    mean, rstd = _empty((2,) + x.shape[:-1], x, torch.float32).unbind()
     if channels == 0:
         mean.zero_(), rstd.zero_()
     _capi.check(_capi.lib.mg_layer_norm(
@@ -242,8 +242,8 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, input_gradient=True,
     rstd = _like(rstd, "rstd", x.shape[:-1], torch.float32)
     weight = _param(weight, "weight", channels, x.dtype)
     params = weight.dtype if weight is not None else torch.float32
-    to_x = _empty(x.shape, x) if input_gradient else None
-    to_weight, to_bias = ((_empty((channels,), x, params) for _ in range(2)) if param_gradients
+    to_x = torch.empty_like(x) if input_gradient else None
+    to_weight, to_bias = (_empty((2, channels), x, params).unbind() if param_gradients
                           else (None, None))
     size = _capi.lib.mg_layer_norm_backward_workspace_size(rows, channels) if param_gradients else 0
     workspace = _workspace(size, x)
@@ -264,7 +264,7 @@ def dropout(x, p, seed=0, offset=0, state=None):
     replayed with other numbers."""
     x = _tensor(x, "x", _DTYPES)
     p, seed, offset, state_ptr = _drop_args(p, seed, offset, state)
-    out = _empty(x.shape, x)
+    out = torch.empty_like(x)
     _capi.check(_capi.lib.mg_dropout(x.numel(), _DTYPES[x.dtype], _ptr(x), p, seed, offset, state_ptr,
                                      _ptr(out), _gr._stream()), "dropout")
     return out
@@ -299,8 +299,8 @@ def encode_types_backward(grad, type_index, table, weight=None, scale=1.0, eps=1
     weight = _param(weight, "weight", channels, table.dtype)
     params = weight.dtype if weight is not None else torch.float32
     p, seed, offset, state_ptr = _drop_args(p, seed, offset, state)
-    to_table = _empty(table.shape, table) if table_gradient else None
-    to_weight, to_bias = ((_empty((channels,), table, params) for _ in range(2)) if param_gradients
+    to_table = torch.empty_like(table) if table_gradient else None
+    to_weight, to_bias = (_empty((2, channels), table, params).unbind() if param_gradients
                           else (None, None))
     size = _capi.lib.mg_encode_types_backward_workspace_size(n, rows, channels)
     workspace = _workspace(size, table)

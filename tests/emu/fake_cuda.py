@@ -177,6 +177,10 @@ def activate():
         return real_to(self, *a, **k)
     torch.Tensor.to = to
     torch.Tensor.record_stream = lambda self, s: None
+    real_new_empty = torch.Tensor.new_empty
+    torch.Tensor.new_empty = lambda self, *a, **k: (
+        on_device(_aligned(torch.Tensor.cpu(real_new_empty(self, *a, **k)))) if isinstance(self, DevTensor)
+        else real_new_empty(self, *a, **k))
 
     def module_cuda(self, *a, **k):
         for m in self.modules():

@@ -288,6 +288,7 @@ inline void compute_here(int&) {}
 inline void lds_barrier() { emu::barrier(); }
 // the lanes of a wave are fibers here and do not run in step: meet
 inline void wave_lds_fence() { uint64_t live; (void)emu::gather(0, &live, "wave_lds_fence"); }
+inline uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return a ^ b ^ c; }
 // conversions of the 16-bit types, to the nearest with ties to even
 inline float half_bits_to_float(uint16_t h) {
   const int e = (h >> 10) & 31, m = h & 1023;
