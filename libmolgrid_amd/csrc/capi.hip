@@ -709,13 +709,10 @@ int mg_embed_types_backward(int ntokens, int nrows, int channels, int dtype, int
     rc = check_workspace(workspace, workspace_bytes,
                          mg_embed_types_backward_workspace_size(ntokens, nrows, channels));
     if (rc != MG_OK) return rc;
-    rc = from_hip(launch_embed_backward(t, grad, scale, scales, grad_table, workspace,
-                                        (hipStream_t)stream));
-    if (rc != MG_OK) return rc;
   }
-  if (to_scales)
-    rc = from_hip(launch_scale_gradient(t, grad, table, grad_scales, (hipStream_t)stream));
-  return rc;
+  return from_hip(launch_embed_backward(t, grad, table, scale, scales, to_table ? grad_table : nullptr,
+                                        to_scales ? grad_scales : nullptr, workspace,
+                                        (hipStream_t)stream));
 }
 
 int mg_layer_norm(int nrows, int channels, int dtype, int param_dtype, const void* x,

@@ -62,23 +62,63 @@ __device__ __forceinline__ Bfloat16 narrow<Bfloat16>(float v) {
   return Bfloat16{float_to_bfloat16_bits(v)};
 }
 
-// VEC elements that are loaded and stored by one instruction (or two, above 16 bytes)
+// VEC elements that are loaded and stored by one instruction (or two, above 16 bytes), kept in
+// whole words: as 16-bit numbers they would take a register each.
 template <typename T, int VEC>
 struct __align__(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
-  T v[VEC];
+  static constexpr int kWords = sizeof(T) * VEC / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float operator[](int i) const;
+  __device__ __forceinline__ void set(const float (&v)[VEC]);
+  __device__ __forceinline__ void zero_unless(bool keep) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = keep ? w[i] : 0u;
+  }
 };
+template <typename T>
+struct __align__(sizeof(T)) Pack<T, 1> {
+  T v;
+  __device__ __forceinline__ float operator[](int) const { return widen(v); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { v = narrow<T>(f[0]); }
+  __device__ __forceinline__ void zero_unless(bool keep) { v = keep ? v : T(); }
+};
+__device__ __forceinline__ float widen_word(uint32_t w, int, float) { return __uint_as_float(w); }
+__device__ __forceinline__ float widen_word(uint32_t w, int upper, Half) {
+  return half_bits_to_float((uint16_t)(upper ? w >> 16 : w));
+}
+__device__ __forceinline__ float widen_word(uint32_t w, int upper, Bfloat16) {
+  return __uint_as_float(upper ? w & 0xFFFF0000u : w << 16);
+}
+__device__ __forceinline__ uint32_t narrow_word(float a, float b, Half) { return floats_to_half_bits(a, b); }
+__device__ __forceinline__ uint32_t narrow_word(float a, float b, Bfloat16) {
+  return floats_to_bfloat16_bits(a, b);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ float Pack<T, VEC>::operator[](int i) const {
+  constexpr int kEach = 4 / sizeof(T);
+  return widen_word(w[i / kEach], i % kEach, T());
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void Pack<T, VEC>::set(const float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    if constexpr (sizeof(T) == 4)
+      w[i] = __float_as_uint(v[i]);
+    else
+      w[i] = narrow_word(v[2 * i], v[2 * i + 1], T());
+  }
+}
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_floats(const T* p, float (&out)[VEC]) {
   const Pack<T, VEC> pack = *reinterpret_cast<const Pack<T, VEC>*>(p);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) out[i] = widen(pack.v[i]);
+  for (int i = 0; i < VEC; ++i) out[i] = pack[i];
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_floats(T* p, const float (&in)[VEC]) {
   Pack<T, VEC> pack;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) pack.v[i] = narrow<T>(in[i]);
+  pack.set(in);
   *reinterpret_cast<Pack<T, VEC>*>(p) = pack;
 }
 

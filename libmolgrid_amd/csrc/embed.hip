@@ -112,45 +112,83 @@ __device__ __forceinline__ void add_token(size_t e, const SumArg& a, float by, u
 constexpr int kTableLds = 64 << 10;   // of a workgroup, so that two share a CU
 constexpr int kTableUnroll = 8;       // tokens of a team in flight
 
-template <typename T, int VEC, int LANES, bool DROP>
+//
+// The tokens of a team go through in rounds of kTableUnroll, a round's loads in flight while the
+// round before it is added.  SCALES: the gradients of the tokens' scales come out on the way
+// (one tile of channels then holds a row), with the table itself in LDS behind the copies.
+template <typename T, int VEC, int LANES, bool DROP, bool SCALES>
 __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T* __restrict__ grad,
-                                                            SumArg a, int share, T* out,
+                                                            SumArg a, int share, const T* __restrict__ table,
+                                                            float* __restrict__ grad_scales, T* out,
                                                             float* partial) {
   HIP_DYNAMIC_SHARED(float, copies);
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const int teams = blockDim.x / LANES;
   const int copy = t.nrows * VEC * LANES;
   float* mine = copies + team * copy + lane;
-  for (int i = 0; i < t.nrows * VEC; ++i) mine[i * LANES] = 0.f;
-  uint64_t seed = 0, offset = 0;
-  if (DROP) drop_key(a.drop, seed, offset);
+  const float* own = copies + teams * copy + lane;
   const int c = (blockIdx.y * LANES + lane) * VEC;
+  const bool inside = c < t.channels;
   const uint32_t begin = blockIdx.x * (uint32_t)share;
   const uint32_t end = min(begin + (uint32_t)share, (uint32_t)t.ntokens);
-  if (c < t.channels)
-    for (uint32_t n0 = begin + team; n0 < end; n0 += teams * kTableUnroll) {
-      uint32_t n[kTableUnroll];
-      int row[kTableUnroll];
-      float by[kTableUnroll], g[kTableUnroll][VEC];
+  struct Round {
+    int row[kTableUnroll];
+    float by[kTableUnroll];
+    Pack<T, VEC> g[kTableUnroll];
+  };
+  const auto fetch = [&](uint32_t n0, Round& r) {
+    uint32_t n[kTableUnroll];
 #pragma unroll
-      for (int u = 0; u < kTableUnroll; ++u) n[u] = n0 + u * teams;
-      token_rows(t, n, end, row);
+    for (int u = 0; u < kTableUnroll; ++u) n[u] = n0 + u * teams;
+    token_rows(t, n, end, r.row);
 #pragma unroll
-      for (int u = 0; u < kTableUnroll; ++u) by[u] = a.scales && n[u] < end ? a.scales[n[u]] : a.scale;
+    for (int u = 0; u < kTableUnroll; ++u) {
+      const uint32_t m = n[u] < end ? n[u] : begin;   // (a token that is there)
+      r.by[u] = a.scales ? a.scales[m] : a.scale;
+      r.g[u] = *reinterpret_cast<const Pack<T, VEC>*>(grad + (size_t)m * t.channels + (inside ? c : 0));
+    }
+  };
+  Round next;
+  fetch(begin + team, next);
+  for (int i = 0; i < t.nrows * VEC; ++i) mine[i * LANES] = 0.f;
+  if (SCALES) {
+    float* to = copies + teams * copy;
+    for (int i = threadIdx.x; i < copy; i += blockDim.x) {
+      const int at = i % LANES * VEC + i / LANES % VEC;
+      to[i] = at < t.channels ? widen(table[(size_t)(i / (LANES * VEC)) * t.channels + at]) : 0.f;
+    }
+    __syncthreads();
+  }
+  uint64_t seed = 0, offset = 0;
+  if (DROP) drop_key(a.drop, seed, offset);
+  for (uint32_t b0 = begin; b0 < end; b0 += teams * kTableUnroll) {
+    const uint32_t n0 = b0 + team;
+    const Round now = next;
+    fetch(n0 + teams * kTableUnroll, next);
 #pragma unroll
-      for (int u = 0; u < kTableUnroll; ++u)
-        if (n[u] < end) load_floats<T, VEC>(grad + (size_t)n[u] * t.channels + c, g[u]);
+    for (int u = 0; u < kTableUnroll; ++u) {
+      const uint32_t n = n0 + u * teams;
+      float g[VEC], dot = 0.f;
 #pragma unroll
-      for (int u = 0; u < kTableUnroll; ++u) {
-        if (row[u] < 0) continue;
+      for (int i = 0; i < VEC; ++i) g[i] = now.g[u][i];
+      if (now.row[u] >= 0 && inside) {
+        const int at = now.row[u] * VEC * LANES;
+        if (SCALES)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) dot = fmaf(g[i], own[at + i * LANES], dot);
         float sum[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] = mine[(row[u] * VEC + i) * LANES];
-        add_token<DROP, VEC>((size_t)n[u] * t.channels + c, a, by[u], seed, offset, g[u], sum);
+        for (int i = 0; i < VEC; ++i) sum[i] = mine[at + i * LANES];
+        add_token<DROP, VEC>((size_t)n * t.channels + c, a, now.by[u], seed, offset, g, sum);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) mine[(row[u] * VEC + i) * LANES] = sum[i];
+        for (int i = 0; i < VEC; ++i) mine[at + i * LANES] = sum[i];
+      }
+      if (SCALES) {
+        dot = team_sum_in_wave<LANES>(dot);
+        if (lane == 0 && n < end) grad_scales[n] = dot;
       }
     }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < copy; i += blockDim.x) {
     float sum = 0.f;
@@ -179,7 +217,7 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
   const int end = min(parts, (wave + 1) * share);
   float sum = 0.f;
   if (e < elements)
-#pragma unroll 8
+#pragma unroll 16
     for (int i = wave * share; i < end; ++i) sum += partial[(size_t)i * elements + e];
   sums[wave][lane] = sum;
   lds_barrier();
@@ -368,7 +406,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
 }
 
 // Tokens of a team in flight, and the first ones of order[begin .. end)
-constexpr int tokens_ahead(int packs) { return packs == 1 ? 8 : 4; }
+constexpr int tokens_ahead(int packs) { return packs == 1 ? 8 : packs <= 4 ? 4 : 2; }
 template <int U>
 __device__ __forceinline__ void first_tokens(const int32_t* order, int begin, int end, uint32_t (&n)[U]) {
 #pragma unroll
@@ -378,12 +416,11 @@ __device__ __forceinline__ void first_tokens(const int32_t* order, int begin, in
 
 // Adds channels c0 + ... of the tokens order[begin .. end) to acc, in that order; `n` are the first of
 // them.  The next ones are read while the gradients of these are under way.
-template <typename T, int VEC, int LANES, int K, bool DROP>
+template <typename T, int VEC, int LANES, int K, bool DROP, int U>
 __device__ __forceinline__ void add_tokens(const TokenArg& t, const T* grad, const SumArg& a,
                                            const int32_t* order, int begin, int end, int c0, int lane,
-                                           uint64_t seed, uint64_t offset,
-                                           uint32_t (&n)[tokens_ahead(K)], float (&acc)[K][VEC]) {
-  constexpr int U = tokens_ahead(K);
+                                           uint64_t seed, uint64_t offset, uint32_t (&n)[U],
+                                           float (&acc)[K][VEC]) {
   for (int i0 = begin; i0 < end; i0 += U) {
     RowPacks<T, VEC, K> g[U];
     uint32_t now[U];
@@ -403,9 +440,10 @@ __device__ __forceinline__ void add_tokens(const TokenArg& t, const T* grad, con
       for (int k = 0; k < K; ++k) {
         float v[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = widen(g[u].pack[k].v[i]);
+        for (int i = 0; i < VEC; ++i) v[i] = g[u].pack[k][i];
         add_token<DROP, VEC>((size_t)now[u] * t.channels + c0 + (k * LANES + lane) * VEC, a, by[u], seed, offset, v,
                              acc[k]);
+        one_after_the_other();
       }
     }
   }
@@ -437,9 +475,10 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(TokenArg t, const T* _
   const int j = slot & 1 ? 0 : (block * kBlock - from + length - 1) / length;
   const int begin = from + j * length, end = min(begin + length, to);
   float acc[K][VEC] = {};
-  uint32_t n[tokens_ahead(K)];
+  constexpr int U = tokens_ahead(K);
+  uint32_t n[U];
   first_tokens(sorted.order, begin, end, n);
-  add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, begin, end, c0, lane, seed, offset, n, acc);
+  add_tokens<T, VEC, LANES, K, DROP, U>(t, grad, a, sorted.order, begin, end, c0, lane, seed, offset, n, acc);
   store_row<float, VEC, LANES, K>(partial + (size_t)slot * t.channels + c0, t.channels - c0, lane, acc);
 }
 
@@ -457,8 +496,11 @@ struct TableNorm {
 // NORM: the sum is the gradient of the row's normed vector, which is taken back through the norm
 // while it is here (a team then holds the whole row); the workgroups stay, and their teams' shares
 // of the gradients of weight and bias are added up at the end.
+constexpr int rows_waves(int elements, bool norm) {   // a SIMD should hold
+  return elements <= 8 ? 4 : elements <= 16 && !norm ? 4 : norm && elements > 16 ? 1 : 2;
+}
 template <typename T, typename O, int VEC, int LANES, int K, bool DROP, bool NORM>
-__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
+__global__ __launch_bounds__((TeamShape<LANES, K>::THREADS), (rows_waves(K * VEC, NORM))) void rows_kernel(
     TokenArg t, const T* __restrict__ grad, SumArg a, Sorted sorted,
     const float* __restrict__ partial, O* __restrict__ out, TableNorm norm) {
   using Shape = TeamShape<LANES, K>;
@@ -477,7 +519,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
 #pragma unroll
       for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.f;
   }
-  constexpr int U = tokens_ahead(K);
+  constexpr int U = NORM ? (K == 1 ? 3 : 2) : K <= 2 ? 4 : 2;   // most rows have a token or two
   const auto bounds = [&](uint32_t row, int& from, int& to) {
     from = row < nrows ? sorted.start[row] : 0;
     to = row < nrows ? sorted.start[row + 1] : 0;
@@ -504,24 +546,25 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
     if (NORM && some)
       load_row<T, VEC, LANES, K>(static_cast<const T*>(norm.table) + (size_t)row * channels, channels, lane, true, x);
     if (to - from <= kDirect) {
-      add_tokens<T, VEC, LANES, K, DROP>(t, grad, a, sorted.order, from, to, c0, lane, seed, offset, n, v);
+      add_tokens<T, VEC, LANES, K, DROP, U>(t, grad, a, sorted.order, from, to, c0, lane, seed, offset, n, v);
     } else {
       const int length = piece_length(to - from), pieces = (to - from + length - 1) / length;
-      for (int j0 = 0; j0 < pieces; j0 += U) {
-        RowPacks<float, VEC, K> p[U];
+      constexpr int P = K == 1 ? (NORM ? 3 : 4) : 2;   // pieces in flight
+      for (int j0 = 0; j0 < pieces; j0 += P) {
+        RowPacks<float, VEC, K> p[P];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < P; ++u) {
           if (j0 + u >= pieces) break;
           load_row<float, VEC, LANES, K>(partial + (size_t)piece_slot(from, length, j0 + u) * t.channels + c0,
                                          channels, lane, true, p[u]);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < P; ++u) {
           if (j0 + u >= pieces) break;
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[k][i] += p[u].pack[k].v[i];
+            for (int i = 0; i < VEC; ++i) v[k][i] += p[u].pack[k][i];
         }
       }
     }
@@ -531,7 +574,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void rows_kernel(
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) h[k][i] = some ? norm.scale * widen(x.pack[k].v[i]) : 0.f;
+        for (int i = 0; i < VEC; ++i) h[k][i] = some ? norm.scale * x.pack[k][i] : 0.f;
       float mean, rstd;
       team_stats<VEC, LANES, K>(h, channels, lane, norm.norm.eps, slots[0], slots[1], mean, rstd);
       float both[2] = {0.f, 0.f};
@@ -655,9 +698,10 @@ SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   return l;
 }
 
+// scales_done: whether the gradients of the scales (if any are wanted) came out as well
 template <typename T, typename O, bool DROP>
-hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, void* out,
-                    float* partial, hipStream_t stream) {
+hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, const void* table, float* grad_scales,
+                    bool* scales_done, void* out, float* partial, hipStream_t stream) {
   with_packs_of<T>(t.channels, address(grad), [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
     with_lanes<VEC>(t.channels / VEC, [&](auto lanes) {
@@ -665,10 +709,19 @@ hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, void* 
       const int column_blocks = (t.channels + LANES * VEC - 1) / (LANES * VEC);
       const FewRowsPlan p = few_rows_plan(t.ntokens, t.nrows, VEC, LANES, column_blocks);
       const bool direct = p.parts == 1 && std::is_same<T, O>::value;
-      hipLaunchKernelGGL((few_rows_kernel<T, VEC, LANES, DROP>), dim3(p.parts, column_blocks),
-                         dim3(p.waves * kWave), (size_t)p.waves * 256 * t.nrows * VEC, stream, t,
-                         (const T*)grad, a, p.share, direct ? (T*)out : nullptr,
-                         direct ? nullptr : partial);
+      const size_t copies = (size_t)p.waves * 256 * t.nrows * VEC;
+      const size_t own = (size_t)t.nrows * VEC * LANES * sizeof(float);
+      const dim3 grid(p.parts, column_blocks), block(p.waves * kWave);
+      if (!DROP && grad_scales && column_blocks == 1 && copies + own <= kTableLds) {
+        if (scales_done) *scales_done = true;
+        hipLaunchKernelGGL((few_rows_kernel<T, VEC, LANES, DROP, !DROP>), grid, block, copies + own, stream, t,
+                           (const T*)grad, a, p.share, (const T*)table, grad_scales, direct ? (T*)out : nullptr,
+                           direct ? nullptr : partial);
+      } else {
+        hipLaunchKernelGGL((few_rows_kernel<T, VEC, LANES, DROP, false>), grid, block, copies, stream, t,
+                           (const T*)grad, a, p.share, (const T*)table, grad_scales, direct ? (T*)out : nullptr,
+                           direct ? nullptr : partial);
+      }
       if (direct) return;
       const size_t elements = (size_t)t.nrows * t.channels;
       hipLaunchKernelGGL((sum_tables_kernel<O>), dim3((unsigned)((elements + kWave - 1) / kWave)),
@@ -730,7 +783,7 @@ hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, voi
                          shared, stream, t, (const T*)grad, a, sorted, partial, (O*)out, norm);
     };
     if constexpr (NORM)
-      with_sum_team<VEC>(packs, [&](auto shape) { rows(shape, kRowParts, 1); });
+      with_team<VEC>(packs, [&](auto shape) { rows(shape, kRowParts, 1); });
     else
       with_tile<VEC, 4>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
   });
@@ -775,22 +828,27 @@ hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const
 #undef MG_CALL
 }
 
-hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scale,
-                                 const float* scales, void* grad_table, void* workspace,
-                                 hipStream_t stream) {
-  const SumArg a{scale, scales, DropArg()};
-#define MG_CALL(T)                                                                                 \
-  t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)                       \
-  : t.nrows <= kFewRows                                                                            \
-      ? few_rows<T, T, false>(t, grad, a, grad_table, (float*)workspace, stream)                   \
-      : sorted_rows<T, T, false, false>(t, grad, a, grad_table, workspace, TableNorm(), stream)
-  MG_FOR_TYPE(t.dtype, MG_CALL);
-#undef MG_CALL
+namespace {
+template <typename T>
+hipError_t embed_backward(const TokenArg& t, const void* grad, const void* table, const SumArg& a,
+                          void* grad_table, float* grad_scales, void* workspace, hipStream_t stream) {
+  hipError_t e = hipSuccess;
+  bool scales_done = false;
+  if (grad_table && t.nrows > 0 && t.channels > 0)
+    e = t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)
+        : t.nrows <= kFewRows
+            ? few_rows<T, T, false>(t, grad, a, table, grad_scales, &scales_done, grad_table, (float*)workspace, stream)
+            : sorted_rows<T, T, false, false>(t, grad, a, grad_table, workspace, TableNorm(), stream);
+  if (e != hipSuccess || !grad_scales || t.ntokens == 0 || scales_done) return e;
+  return scale_gradient<T>(t, grad, table, grad_scales, stream);
 }
+}  // namespace
 
-hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
-                                 float* grad_scales, hipStream_t stream) {
-#define MG_CALL(T) scale_gradient<T>(t, grad, table, grad_scales, stream)
+hipError_t launch_embed_backward(const TokenArg& t, const void* grad, const void* table, float scale,
+                                 const float* scales, void* grad_table, float* grad_scales,
+                                 void* workspace, hipStream_t stream) {
+  const SumArg a{scale, scales, DropArg()};
+#define MG_CALL(T) embed_backward<T>(t, grad, table, a, grad_table, grad_scales, workspace, stream)
   MG_FOR_TYPE(t.dtype, MG_CALL);
 #undef MG_CALL
 }
@@ -829,7 +887,8 @@ hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad
   hipError_t e = t.nrows == 0 ? hipSuccess
                  : t.ntokens == 0 ? zero<float>(sums, (size_t)t.nrows * t.channels, stream)
                  : t.nrows <= kFewRows
-                     ? few_rows<T, float, true>(t, grad, a, sums, (float*)(workspace + l.rest), stream)
+                     ? few_rows<T, float, true>(t, grad, a, nullptr, nullptr, nullptr, sums, (float*)(workspace + l.rest),
+                                                stream)
                      : sorted_rows<T, float, true, false>(t, grad, a, sums, workspace + l.rest, TableNorm(), stream);
   if (e != hipSuccess) return e;
   return launch_table_norm_backward(n, sums, table, scale, grad_table, grad_weight, grad_bias, params, stream);

@@ -39,6 +39,10 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 // moving LDS accesses across the point.
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_wave_barrier(); }
 
+// Keeps the compiler's scheduler from mixing what comes before with what comes after: independent
+// pieces of work done side by side need the registers of all of them.
+__device__ __forceinline__ void one_after_the_other() { __builtin_amdgcn_sched_barrier(0); }
+
 // a ^ b ^ c
 __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
   return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
@@ -53,6 +57,19 @@ __device__ __forceinline__ uint16_t float_to_half_bits(float v) {
 }
 __device__ __forceinline__ uint16_t float_to_bfloat16_bits(float v) {
   return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+// Two at once, the first in the low half.
+__device__ __forceinline__ uint32_t floats_to_half_bits(float a, float b) {
+  typedef float Floats __attribute__((ext_vector_type(2)));
+  typedef _Float16 Halves __attribute__((ext_vector_type(2)));
+  const Floats v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, Halves));
+}
+__device__ __forceinline__ uint32_t floats_to_bfloat16_bits(float a, float b) {
+  typedef float Floats __attribute__((ext_vector_type(2)));
+  typedef __bf16 Halves __attribute__((ext_vector_type(2)));
+  const Floats v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, Halves));
 }
 
 }  // namespace mg

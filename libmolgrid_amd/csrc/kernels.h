@@ -120,11 +120,9 @@ hipError_t launch_interpolate(const InterpArg& p, int nbatch, const Vec3Arg& in_
 hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const float* scales,
                         void* out, hipStream_t stream);
 size_t embed_backward_workspace_bytes(int ntokens, int nrows, int channels);
-hipError_t launch_embed_backward(const TokenArg& t, const void* grad, float scale,
-                                 const float* scales, void* grad_table, void* workspace,
-                                 hipStream_t stream);
-hipError_t launch_scale_gradient(const TokenArg& t, const void* grad, const void* table,
-                                 float* grad_scales, hipStream_t stream);
+hipError_t launch_embed_backward(const TokenArg& t, const void* grad, const void* table, float scale,
+                                 const float* scales, void* grad_table, float* grad_scales,
+                                 void* workspace, hipStream_t stream);
 
 hipError_t launch_norm(const NormArg& a, const void* x, const void* bias, void* out, float* means,
                        float* rstds, hipStream_t stream);

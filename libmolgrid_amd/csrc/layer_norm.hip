@@ -100,7 +100,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        v[k][i] = ENCODE ? scale * widen(packs.pack[k].v[i]) : widen(packs.pack[k].v[i]);
+        v[k][i] = ENCODE ? scale * packs.pack[k][i] : packs.pack[k][i];
     float mean, rstd;
     team_stats<VEC, LANES, K>(v, channels, lane, a.eps, slots[0], slots[1], mean, rstd);
     if (n >= nrows) continue;
@@ -125,7 +125,79 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
   }
 }
 
-// Rows wider than any team (more than 16,384 channels): a workgroup goes over the row three times,
+// ENCODE with a table of few rows: every workgroup norms the table once, into LDS, and goes through
+// the result in groups of eight elements, each with one counter of the generator and one store,
+// whatever the channels are.
+constexpr int kFewRowsFloats = 8192;   // of a table: 32 KB
+constexpr size_t kFewRowsBlocks = 1024;
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void few_rows_encode_kernel(
+    const T* __restrict__ table, TokenArg t, float scale, NormArg a, const void* __restrict__ bias,
+    DropArg arg, uint32_t step_tokens, int step_channels, T* __restrict__ out) {
+  HIP_DYNAMIC_SHARED(float, vectors);   // [nrows][channels]
+  uint64_t seed, offset;
+  drop_key(arg, seed, offset);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, channels = t.channels;
+  const bool is_float = a.param_dtype == MG_FLOAT32;
+  for (int row = wave; row < t.nrows; row += kWaves) {
+    float* v = vectors + row * channels;
+    float sum = 0.f, squares = 0.f;
+    for (int c = lane; c < channels; c += kWave) {
+      v[c] = scale * widen(table[(size_t)row * channels + c]);
+      sum += v[c];
+    }
+    const float mean = lanes_sum(sum) / channels;
+    for (int c = lane; c < channels; c += kWave) {   // (every lane its own elements)
+      const float d = v[c] - mean;
+      squares = fmaf(d, d, squares);
+    }
+    const float rstd = 1.f / sqrtf(lanes_sum(squares) / channels + a.eps);
+    for (int c = lane; c < channels; c += kWave)
+      v[c] = fmaf((v[c] - mean) * rstd, param_at<T>(a.weight, is_float, c, 1.f), param_at<T>(bias, is_float, c, 0.f));
+  }
+  __syncthreads();
+  const size_t total = (size_t)t.ntokens * channels, step = (size_t)gridDim.x * kThreads * 8;
+  size_t e = ((size_t)blockIdx.x * kThreads + threadIdx.x) * 8;
+  uint32_t n = (uint32_t)(e / channels);
+  int c = (int)(e % channels);
+  for (; e < total; e += step) {
+    float v[8];
+    if (WHOLE) {   // rows are whole groups
+      const int row = token_row(t, n);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = row < 0 ? 0.f : vectors[row * channels + c + i];
+    } else {
+      uint32_t m = n;
+      int at = c, row = token_row(t, m);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = row < 0 ? 0.f : vectors[row * channels + at];
+        if (++at == channels) {
+          at = 0;
+          ++m;
+          row = m < (uint32_t)t.ntokens ? token_row(t, m) : -1;
+        }
+      }
+    }
+    drop<8>(e, arg, seed, offset, v);
+    if (WHOLE || (e + 8 <= total && (reinterpret_cast<uintptr_t>(out) & 15) == 0)) {
+      store_floats<T, 8>(out + e, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (e + i < total) out[e + i] = narrow<T>(v[i]);
+    }
+    n += step_tokens;
+    c += step_channels;
+    if (c >= channels) {
+      c -= channels;
+      ++n;
+    }
+  }
+}
+
+// Rows wider than any team (more than 8,192 channels): a workgroup goes over the row three times,
 // which stays in the caches.
 template <typename T, bool ENCODE>
 __global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenArg tokens,
@@ -164,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenAr
 // Backward: a team holds the rows of x and of the gradient, writes dx, and a lane adds its share of
 // dw and db up over all rows that its team takes.  G: type of the gradient; TABLE: x is a scaled
 // table, whose statistics are computed here.
-constexpr int kParts = 512;
+constexpr int kParts = 512, kNarrowParts = 1024;   // workgroups that share the rows
 
 template <typename T, typename G, int VEC, int LANES, int K, bool TABLE>
 __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_kernel(
@@ -211,7 +283,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) h[k][i] = TABLE ? scale * widen(px.pack[k].v[i]) : widen(px.pack[k].v[i]);
+      for (int i = 0; i < VEC; ++i) h[k][i] = TABLE ? scale * px.pack[k][i] : px.pack[k][i];
     if (TABLE) {
       team_stats<VEC, LANES, K>(h, channels, lane, a.eps, slots[2], slots[3], mean, rstd);
       mean = 0.f;   // (taken out already)
@@ -221,7 +293,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float g = widen(pg.pack[k].v[i]);
+        const float g = pg.pack[k][i];
         h[k][i] = (h[k][i] - mean) * rstd;
         const float q = g * w[k][i];
         both[0] += q;
@@ -240,7 +312,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
       float d[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float q = widen(pg.pack[k].v[i]) * w[k][i];
+        const float q = pg.pack[k][i] * w[k][i];
         d[i] = factor * (q - mean_q - h[k][i] * mean_qh);
       }
       store_floats<T, VEC>(grad_x + (size_t)n * channels + c, d);
@@ -312,7 +384,7 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_partials_kernel(
   const int end = min(parts, (wave + 1) * share);
   float sum = 0.f;
   if (c < columns)
-#pragma unroll 8
+#pragma unroll 16
     for (int i = wave * share; i < end; ++i) sum += partial[(size_t)i * columns + c];
   sums[wave][lane] = sum;
   lds_barrier();
@@ -337,6 +409,21 @@ template <typename T, bool ENCODE>
 hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x, const void* bias,
                 const DropArg& drop, void* out, float* means, float* rstds, hipStream_t stream) {
   const uint32_t nrows = (uint32_t)(ENCODE ? t.ntokens : a.nrows);
+  if (ENCODE && t.nrows <= t.ntokens && (size_t)t.nrows * t.channels <= kFewRowsFloats) {
+    const size_t groups = ((size_t)t.ntokens * t.channels + 7) / 8;
+    const size_t all = (groups + kThreads - 1) / kThreads, blocks = all < kFewRowsBlocks ? all : kFewRowsBlocks;
+    const size_t step = blocks * kThreads * 8, shared = (size_t)t.nrows * t.channels * sizeof(float);
+    const bool whole = t.channels % 8 == 0 && address(out) % 16 == 0;
+    const uint32_t step_tokens = (uint32_t)(step / t.channels);
+    const int step_channels = (int)(step % t.channels);
+    if (whole)
+      hipLaunchKernelGGL((few_rows_encode_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), shared, stream,
+                         (const T*)x, t, scale, a, bias, drop, step_tokens, step_channels, (T*)out);
+    else
+      hipLaunchKernelGGL((few_rows_encode_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), shared, stream,
+                         (const T*)x, t, scale, a, bias, drop, step_tokens, step_channels, (T*)out);
+    return hipGetLastError();
+  }
   const auto with_packs = [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
     return with_team<VEC>((a.channels + VEC - 1) / VEC, [&](auto shape) {
@@ -358,12 +445,12 @@ hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x,
   return hipGetLastError();
 }
 
-// Workgroups that share the rows, each with its row of partial sums: as many as fill the chip, but
-// no more than rows for eight rounds where the sums' own traffic (8 bytes a channel and workgroup)
-// would not be small beside that of the rows.
+// Workgroups that share the rows, each with its row of partial sums (8 bytes a channel): as many as
+// fill the chip, more of them where rows are narrow and many share a workgroup.
 int norm_parts(int nrows, int teams) {
   const size_t rounds = ((size_t)nrows + teams - 1) / teams;
-  return (int)(rounds < kParts ? rounds : kParts);
+  const size_t most = teams > 4 ? kNarrowParts : kParts;
+  return (int)(rounds < most ? rounds : most);
 }
 
 template <typename T, typename G, bool TABLE>
@@ -409,8 +496,10 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
 }  // namespace
 
 size_t norm_backward_workspace_bytes(int nrows, int channels) {
-  // (a team of one row at a time has the most workgroups)
-  return (size_t)norm_parts(nrows, 1) * 2 * channels * sizeof(float);
+  size_t parts = 0;   // (whichever team takes the rows)
+  for (int teams = 1; teams <= 64; teams *= 2)
+    if ((size_t)norm_parts(nrows, teams) > parts) parts = norm_parts(nrows, teams);
+  return parts * 2 * channels * sizeof(float);
 }
 
 #define MG_FOR_TYPE(dtype, FN)                \

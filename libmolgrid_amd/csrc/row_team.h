@@ -17,19 +17,21 @@ struct TeamShape {
   static constexpr int WAVES = THREADS / kWave;
 };
 
-constexpr int kMostTeamChannels = 16384;   // of rows that a team can hold
+constexpr int kMostTeamChannels = 8192;   // of rows that a team can hold
 
-// Calls f with the shape for rows of `packs` packs: the narrowest team that holds them, in which a
-// lane holds up to 32 elements of 16-bit types, 16 of any other.  False: no team is wide enough.
+// Calls f with the shape for rows of `packs` packs.  Few elements a lane (up to 32 of 16-bit types, 16
+// of any other) leave room for many waves, whose loads hide one another; four-wave teams pay with a
+// barrier a sum.  1001 channels of float16, one element a pack: 64 lanes of 16 packs take 16 us where
+// 256 lanes of four take 8 (4099 rows).  False: no team is wide enough.
 template <int VEC, typename F>
 bool with_team(int packs, F f) {
   if constexpr (VEC == 1) {
     if (packs <= 16) return f(TeamShape<16, 1>()), true;
     if (packs <= 64) return f(TeamShape<64, 1>()), true;
     if (packs <= 256) return f(TeamShape<64, 4>()), true;
-    if (packs <= 1024) return f(TeamShape<64, 16>()), true;
+    if (packs <= 1024) return f(TeamShape<256, 4>()), true;
     if (packs <= 4096) return f(TeamShape<256, 16>()), true;
-    if (packs <= 16384) return f(TeamShape<1024, 16>()), true;
+    if (packs <= 8192) return f(TeamShape<1024, 8>()), true;
   } else {
     if (packs <= 4) return f(TeamShape<4, 1>()), true;
     if (packs <= 8) return f(TeamShape<8, 1>()), true;
@@ -37,25 +39,13 @@ bool with_team(int packs, F f) {
     if (packs <= 32) return f(TeamShape<32, 1>()), true;
     if (packs <= 64) return f(TeamShape<64, 1>()), true;
     if (packs <= 128) return f(TeamShape<64, 2>()), true;
-    if (packs <= 256) return f(TeamShape<64, 4>()), true;
+    if (packs <= 256) return f(TeamShape<256, 1>()), true;
     if (packs <= 512) return f(TeamShape<256, 2>()), true;
     if (packs <= 1024) return f(TeamShape<256, 4>()), true;
-    if (packs <= 4096 * 4 / VEC) return f(TeamShape<1024, 16 / VEC>()), true;
+    if constexpr (VEC == 4)
+      if (packs <= 2048) return f(TeamShape<1024, 2>()), true;
   }
   return false;
-}
-
-// The same for sums over scattered rows, whose loads wait for one another: wider teams, so that a
-// lane has as many rows in flight as it can.
-template <int VEC, typename F>
-bool with_sum_team(int packs, F f) {
-  if constexpr (VEC == 1) {
-    if (packs > 64 && packs <= 256) return f(TeamShape<256, 1>()), true;
-    if (packs > 256 && packs <= 1024) return f(TeamShape<256, 4>()), true;
-  } else {
-    if (packs > 64 && packs <= 256) return f(TeamShape<256, 1>()), true;
-  }
-  return with_team<VEC>(packs, f);
 }
 
 // Teams of a wave or less for rows that are gone through in tiles of up to `most` packs a lane
@@ -135,10 +125,7 @@ __device__ __forceinline__ void load_row(const T* row, int channels, int lane, b
     out.pack[k] = *reinterpret_cast<const Pack<T, VEC>*>(row + (c < channels ? c : 0));
   }
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (!(live && (k * LANES + lane) * VEC < channels)) out.pack[k].v[i] = T();
+  for (int k = 0; k < K; ++k) out.pack[k].zero_unless(live && (k * LANES + lane) * VEC < channels);
 }
 
 // A lane's share of a parameter (float or of type T, or absent)
@@ -282,17 +269,22 @@ __device__ __forceinline__ void drop(size_t e, const DropArg& a, uint64_t seed, 
                                      float (&v)[VEC]) {
   if (a.limit == 0) return;
   const Words4 words = philox(e >> 3, offset, seed);
+  const uint32_t upper = 0u - ((uint32_t)(e >> 2) & 1u);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
+    // (selections by bits: an index that depends on e would put the words into memory)
     uint32_t half;
     if (VEC == 8) {
       half = drop_half(words, i);
     } else if (VEC == 4) {
-      const uint32_t w = (e & 4) ? words.w[2 + i / 2] : words.w[i / 2];
+      const uint32_t w = words.w[i / 2] ^ ((words.w[i / 2] ^ words.w[2 + i / 2]) & upper);
       half = i & 1 ? w >> 16 : w & 0xFFFFu;
     } else {
-      const uint32_t pair = (e & 4) ? ((e & 2) ? words.w[3] : words.w[2]) : ((e & 2) ? words.w[1] : words.w[0]);
-      half = (e & 1) ? pair >> 16 : pair & 0xFFFFu;
+      const uint32_t odd = 0u - ((uint32_t)(e >> 1) & 1u);
+      const uint32_t w0 = words.w[0] ^ ((words.w[0] ^ words.w[2]) & upper);
+      const uint32_t w1 = words.w[1] ^ ((words.w[1] ^ words.w[3]) & upper);
+      const uint32_t w = w0 ^ ((w0 ^ w1) & odd);
+      half = (e & 1) ? w >> 16 : w & 0xFFFFu;
     }
     v[i] = half >= a.limit ? v[i] * a.factor : 0.f;
   }

@@ -288,6 +288,7 @@ inline void compute_here(int&) {}
 inline void lds_barrier() { emu::barrier(); }
 // the lanes of a wave are fibers here and do not run in step: meet
 inline void wave_lds_fence() { uint64_t live; (void)emu::gather(0, &live, "wave_lds_fence"); }
+inline void one_after_the_other() {}
 inline uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return a ^ b ^ c; }
 // conversions of the 16-bit types, to the nearest with ties to even
 inline float half_bits_to_float(uint16_t h) {
@@ -311,4 +312,6 @@ inline uint16_t float_to_bfloat16_bits(float f) {
   if (f != f) return (uint16_t)((u >> 16) | 0x40u);
   return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
+inline uint32_t floats_to_half_bits(float a, float b) { return float_to_half_bits(a) | (uint32_t)float_to_half_bits(b) << 16; }
+inline uint32_t floats_to_bfloat16_bits(float a, float b) { return float_to_bfloat16_bits(a) | (uint32_t)float_to_bfloat16_bits(b) << 16; }
 }  // namespace mg
