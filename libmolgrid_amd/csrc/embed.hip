@@ -14,6 +14,9 @@
 #include "kernels.h"
 #include "row_team.h"
 
+#ifndef MG_K
+#define MG_K 4
+#endif
 namespace mg {
 namespace {
 
@@ -228,22 +231,21 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
 
 // ---- any table: the tokens sorted by row ----------------------------------------------------------
 //
-// One launch sorts: a workgroup owns a range of rows, reads every index and keeps those of its range.
-// First it counts its rows' tokens, and the tokens of lower rows, which is where its part of the
-// order begins; then it goes again through the steps of 64 tokens that held one of its own and writes
-// those in place.  Each of its waves goes through a piece of the tokens of its own, with counters of
-// its own, so the order within a row is that of the tokens.  All workgroups read all indices (out of
-// the L2 after the first), which costs less than the launches of a sort by digits for up to about
-// 2^18 tokens.
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kSortRange = 960;   // most rows of a workgroup: 60 KB of counters
+// Up to kOneLaunchTokens tokens are sorted by one launch (sort_tokens_kernel): a workgroup owns a range
+// of rows, reads every index and keeps those of its range.  Every compute unit reads all indices
+// then, and the workgroup of a frequent row has most of the placing to do: 7 us for 1,000 tokens,
+// 16 us for 16,384, 45 us for 65,536 and 181 us for 262,144 of a vocabulary (131,072 rows).  More
+// tokens are sorted by digits of their row, two launches for each of 9 bits, whose time hardly depends
+// on the tokens.  Both give the same order: rows ascending, and the tokens of a row as they were.
+constexpr int kOneLaunchTokens = 32768;
 
 // A row of up to kDirect tokens is added up by one team.  Longer ones are cut into pieces that
 // start at multiples of their length from the row's start, a multiple of kBlock tokens, so that the
-// tokens of a piece and the pieces of a row, which are added up one after the other, stay balanced.  A piece's sum has slot 2 b + f, where b is the block of kBlock
-// positions of the order that the piece starts in and f whether it is its row's first: of a block's
-// positions at most two start pieces, a first one (its row then holds the block's last position) and
-// a later one (its row then holds the block's first position).
+// tokens of a piece and the pieces of a row, which are added up one after the other, stay balanced.
+// A piece's sum has slot 2 b + f, where b is the block of kBlock positions of the order that the piece
+// starts in and f whether it is its row's first: of a block's positions at most two start pieces, a
+// first one (its row then holds the block's last position) and a later one (its row then holds the
+// block's first position).
 constexpr int kBlock = 16, kDirect = 32;
 
 __device__ __forceinline__ int piece_length(int count) {
@@ -254,10 +256,17 @@ __device__ __forceinline__ int piece_slot(int from, int length, int j) {
 }
 
 struct Sorted {
-  int32_t* start;      // [nrows + 1]: where a row's tokens begin in order
-  int32_t* order;      // [ntokens]
-  int32_t* piece_row;  // [2 blocks]: row of the piece in a slot, or -1 (unwritten past the last token)
+  int32_t* start;   // [nrows + 1]: where a row's tokens begin in order
+  int32_t* order;   // [ntokens]; start[nrows] of them have a row
+  int32_t* row;     // [ntokens]: the row of the token at a position of order
 };
+
+// The one launch: first a workgroup counts its rows' tokens, and the tokens of lower rows, which is
+// where its part of the order begins; then it goes again through the steps of 64 tokens that held one
+// of its own and writes those in place.  Each of its waves goes through a piece of the tokens of its
+// own, with counters of its own, so the order within a row is that of the tokens.
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kSortRange = 960;   // most rows of a workgroup: 60 KB of counters
 
 __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
 #pragma unroll
@@ -274,7 +283,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
                                                                    int range, Sorted sorted) {
   HIP_DYNAMIC_SHARED(int, count);   // [kSortWaves][range]
   __shared__ int sums[kSortWaves];
-  __shared__ int last;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int row0 = blockIdx.x * range, rows = min(range, nrows - row0);
   for (int i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) count[i] = 0;
@@ -325,38 +333,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
       count[w * range + r] = at;
       at += c;
     }
-    if (r == rows - 1) last = at;
     if (row0 + r == nrows - 1) sorted.start[nrows] = at;
-  }
-  __syncthreads();
-  // Slots of the blocks of the order that this workgroup's rows hold the first or last position of:
-  // a thread does those of its row, a wave those of a row that is cut.
-  if (sorted.piece_row) {
-    for (int i = threadIdx.x; i < rows; i += kSortThreads) {
-      const int from = count[i], to = i + 1 < rows ? count[i + 1] : last;
-      if (to - from > kDirect) continue;
-      for (int b = from / kBlock; b * kBlock < to; ++b) {
-        if (b * kBlock >= from) sorted.piece_row[2 * b] = -1;
-        if (b * kBlock + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = -1;
-      }
-    }
-    for (int i0 = wave * kWave; i0 < rows; i0 += kSortWaves * kWave) {
-      const int i1 = i0 + lane, end_of = i1 + 1 < rows ? count[min(i1 + 1, rows - 1)] : last;
-      unsigned long long cut = __ballot(i1 < rows && end_of - count[min(i1, rows - 1)] > kDirect);
-      for (; cut; cut &= cut - 1) {
-        const int i = i0 + (int)__builtin_ctzll(cut);
-        const int from = count[i], to = i + 1 < rows ? count[i + 1] : last;
-        const int length = piece_length(to - from);
-        for (int b = from / kBlock + lane; b * kBlock < to; b += kWave) {
-          const int first = b * kBlock;
-          if (first >= from) {
-            const int j = (first - from + length - 1) / length, p = from + j * length;
-            sorted.piece_row[2 * b] = j > 0 && p < to && p < first + kBlock ? row0 + i : -1;
-          }
-          if (first + kBlock - 1 < to) sorted.piece_row[2 * b + 1] = first <= from ? row0 + i : -1;
-        }
-      }
-    }
   }
   __syncthreads();
   const unsigned long long below = (1ull << lane) - 1;
@@ -372,6 +349,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
       if (inside && r == first) {
         const int rank = __popcll(same & below);
         sorted.order[to + rank] = (int32_t)n;
+        sorted.row[to + rank] = row;
         if (rank == 0) mine[first] = to + __popcll(same);
       }
       wave_lds_fence();
@@ -379,13 +357,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
     }
   };
   constexpr int kTogether = 4;
-  if (steps > 64 * kWave) {   // (more than four million tokens: more steps than bits)
-    for (uint32_t s = 0; s < steps; ++s) {
-      const uint32_t n = begin + s * kWave + lane;
-      place(n, fetch(n));
-    }
-    return;
-  }
   for (uint32_t l = 0; l * 64 < steps; ++l) {
     uint64_t bits = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)held, (int)l) |
                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(held >> 32), (int)l) << 32;
@@ -402,6 +373,124 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) place(n[u], row[u]);
     }
+  }
+}
+
+// By digits: the tokens of a tile are counted by their digit, then every tile's workgroup works out
+// where each of its digits begins from all tiles' counts, ranks its tokens (those of a wave by the
+// lanes of equal digit, those of its waves one after the other) and moves them.  FIRST: the rows come
+// from the indices; a token without a row gets the row behind the last one.
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kTile = 4096, kTileSteps = kTile / kSortThreads;
+
+template <bool FIRST>
+__device__ __forceinline__ uint32_t tile_row(const TokenArg& t, const int32_t* rows, uint32_t i) {
+  if (!FIRST) return (uint32_t)rows[i];
+  const int row = token_row(t, i);
+  return row < 0 ? (uint32_t)t.nrows : (uint32_t)row;
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void count_digits_kernel(TokenArg t, const int32_t* __restrict__ rows,
+                                                                    int shift, int32_t* __restrict__ counts) {
+  __shared__ int count[kDigits];
+  for (int i = threadIdx.x; i < kDigits; i += kSortThreads) count[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const uint32_t i = blockIdx.x * (uint32_t)kTile + k * kSortThreads + threadIdx.x;
+    if (i < (uint32_t)t.ntokens) atomicAdd(&count[tile_row<FIRST>(t, rows, i) >> shift & (kDigits - 1)], 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kDigits; i += kSortThreads) counts[(size_t)blockIdx.x * kDigits + i] = count[i];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void move_digits_kernel(
+    TokenArg t, const int32_t* __restrict__ rows, const int32_t* __restrict__ order, int shift,
+    const int32_t* __restrict__ counts, int32_t* __restrict__ to_rows, int32_t* __restrict__ to_order) {
+  __shared__ int count[kSortWaves][kDigits];   // of a wave's tokens, then where they go
+  __shared__ int totals[2][kDigits], befores[2][kDigits], sums[kSortWaves];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) (&count[0][0])[i] = 0;
+  // the tiles' counts of a digit: all of them, and those of the tiles before this one
+  const int digit = threadIdx.x % kDigits, half = threadIdx.x / kDigits;
+  int total = 0, before = 0;
+#pragma unroll 8
+  for (int k = half; k < (int)gridDim.x; k += kSortThreads / kDigits) {
+    const int v = counts[(size_t)k * kDigits + digit];
+    total += v;
+    before += k < (int)blockIdx.x ? v : 0;
+  }
+  totals[half][digit] = total;
+  befores[half][digit] = before;
+  uint32_t row[kTileSteps];
+  int token[kTileSteps], rank[kTileSteps];
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const uint32_t i = blockIdx.x * (uint32_t)kTile + (wave * kTileSteps + k) * kWave + lane;
+    const bool there = i < (uint32_t)t.ntokens;
+    row[k] = there ? tile_row<FIRST>(t, rows, i) : 0xFFFFFFFFu;
+    token[k] = FIRST || !there ? (int)i : order[i];
+  }
+  __syncthreads();
+  const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const bool there = row[k] != 0xFFFFFFFFu;
+    const int d = row[k] >> shift & (kDigits - 1);
+    unsigned long long same = __ballot(there);   // the lanes of this lane's digit
+#pragma unroll
+    for (int b = 0; b < kDigitBits; ++b) {
+      const unsigned long long set = __ballot(d >> b & 1);
+      same &= d >> b & 1 ? set : ~set;
+    }
+    const int at = count[wave][d];
+    rank[k] = at + __popcll(same & below);
+    wave_lds_fence();
+    if (there && (same & below) == 0) count[wave][d] = at + __popcll(same);
+    wave_lds_fence();
+  }
+  __syncthreads();
+  int mine = 0;   // threads of the first half: a digit each
+  if (half == 0) mine = totals[0][digit] + totals[1][digit];
+  const int through = wave_inclusive_sum(mine, lane);
+  if (lane == kWave - 1) sums[wave] = through;
+  __syncthreads();
+  if (half == 0) {
+    int at = through - mine + befores[0][digit] + befores[1][digit];
+    for (int w = 0; w < wave; ++w) at += sums[w];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = count[w][digit];
+      count[w][digit] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k)
+    if (row[k] != 0xFFFFFFFFu) {
+      const int to = count[wave][row[k] >> shift & (kDigits - 1)] + rank[k];
+      to_rows[to] = (int32_t)row[k];
+      to_order[to] = token[k];
+    }
+}
+
+// Where the rows begin, out of the sorted tokens' rows: a thread a position (and one behind the last)
+// fills in the rows that begin there, a wave those of a wide gap.
+__global__ __launch_bounds__(kThreads) void row_starts_kernel(TokenArg t, Sorted sorted) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const uint32_t i = blockIdx.x * (uint32_t)kThreads + threadIdx.x, ntokens = (uint32_t)t.ntokens;
+  const bool there = i <= ntokens;
+  const int from = there && i > 0 ? sorted.row[i - 1] + 1 : 0;   // first row to fill in
+  const int to = !there ? 0 : i < ntokens ? sorted.row[i] : t.nrows;
+  const bool wide = there && to - from >= 8;
+  if (there && !wide)
+    for (int r = from; r <= to; ++r) sorted.start[r] = (int32_t)i;
+  for (unsigned long long left = __ballot(wide); left; left &= left - 1) {
+    const int who = (int)__builtin_ctzll(left);
+    const int a = __builtin_amdgcn_readlane(from, who), b = __builtin_amdgcn_readlane(to, who);
+    const int at = __builtin_amdgcn_readlane((int)i, who);
+    for (int64_t r = (int64_t)a + lane; r <= b; r += kWave) sorted.start[r] = at;
   }
 }
 
@@ -466,14 +555,17 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(TokenArg t, const T* _
   const int lane = threadIdx.x % LANES;
   const int slot = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const int block = slot / 2, c0 = blockIdx.y * LANES * K * VEC;
-  if ((int64_t)block * kBlock + (slot & 1 ? kBlock - 1 : 0) >= sorted.start[t.nrows]) return;
-  const int row = sorted.piece_row[slot];
-  if (row < 0) return;
+  const int64_t position = (int64_t)block * kBlock + (slot & 1 ? kBlock - 1 : 0);
+  if (position >= sorted.start[t.nrows]) return;
+  const int row = sorted.row[position], from = sorted.start[row], to = sorted.start[row + 1];
+  const int first = block * kBlock, length = piece_length(to - from);
+  if (to - from <= kDirect) return;
+  // the row's first piece, if it starts in this block, or the one that does, if it is a later one
+  const int j = slot & 1 ? 0 : (first - from + length - 1) / length;
+  const int begin = from + j * length, end = min(begin + length, to);
+  if (slot & 1 ? from < first : j == 0 || begin >= to || begin >= first + kBlock) return;
   uint64_t seed = 0, offset = 0;
   if (DROP) drop_key(a.drop, seed, offset);
-  const int from = sorted.start[row], to = sorted.start[row + 1], length = piece_length(to - from);
-  const int j = slot & 1 ? 0 : (block * kBlock - from + length - 1) / length;
-  const int begin = from + j * length, end = min(begin + length, to);
   float acc[K][VEC] = {};
   constexpr int U = tokens_ahead(K);
   uint32_t n[U];
@@ -685,15 +777,20 @@ size_t few_rows_bytes(int ntokens, int nrows, int channels) {
 }
 
 struct SortedLayout {
-  size_t order, piece_row, partial, bytes;   // offsets into the workspace; start is first
-  int slots;
+  size_t order, row, other_order, other_row, counts, partial, bytes;   // offsets; start is first
+  int slots, tiles;
 };
 SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   SortedLayout l;
   l.slots = ntokens > kDirect ? (ntokens + kBlock - 1) / kBlock * 2 : 0;
+  l.tiles = ntokens > kOneLaunchTokens ? (ntokens + kTile - 1) / kTile : 0;
+  const size_t list = round_up((size_t)ntokens * sizeof(int32_t));
   l.order = round_up(((size_t)nrows + 1) * sizeof(int32_t));
-  l.piece_row = l.order + round_up((size_t)ntokens * sizeof(int32_t));
-  l.partial = l.piece_row + round_up((size_t)l.slots * sizeof(int32_t));
+  l.row = l.order + list;
+  l.other_order = l.row + list;
+  l.other_row = l.other_order + (l.tiles ? list : 0);
+  l.counts = l.other_row + (l.tiles ? list : 0);
+  l.partial = l.counts + round_up((size_t)l.tiles * kDigits * sizeof(int32_t));
   l.bytes = l.partial + round_up((size_t)l.slots * channels * sizeof(float));
   return l;
 }
@@ -731,7 +828,32 @@ hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, const 
   return hipGetLastError();
 }
 
-void sort_tokens(const TokenArg& t, const Sorted& sorted, hipStream_t stream) {
+Sorted sort_tokens(const TokenArg& t, const SortedLayout& l, char* base, hipStream_t stream) {
+  const auto list = [&](size_t at) { return reinterpret_cast<int32_t*>(base + at); };
+  const Sorted sorted{list(0), list(l.order), list(l.row)};
+  if (l.tiles) {
+    int passes = 1;   // digits of 0 .. nrows
+    while (passes < 4 && (uint32_t)t.nrows >> (passes * kDigitBits)) ++passes;
+    const Sorted other{nullptr, list(l.other_order), list(l.other_row)};
+    for (int p = 0; p < passes; ++p) {
+      const bool last = (passes - 1 - p) % 2 == 0;   // the last pass ends in `sorted`
+      const Sorted &to = last ? sorted : other, &from = last ? other : sorted;
+      const dim3 grid(l.tiles), block(kSortThreads);
+      if (p == 0) {
+        hipLaunchKernelGGL(count_digits_kernel<true>, grid, block, 0, stream, t, nullptr, 0, list(l.counts));
+        hipLaunchKernelGGL(move_digits_kernel<true>, grid, block, 0, stream, t, nullptr, nullptr, 0,
+                           list(l.counts), to.row, to.order);
+      } else {
+        hipLaunchKernelGGL(count_digits_kernel<false>, grid, block, 0, stream, t, from.row, p * kDigitBits,
+                           list(l.counts));
+        hipLaunchKernelGGL(move_digits_kernel<false>, grid, block, 0, stream, t, from.row, from.order,
+                           p * kDigitBits, list(l.counts), to.row, to.order);
+      }
+    }
+    hipLaunchKernelGGL(row_starts_kernel, dim3(((unsigned)t.ntokens + kThreads) / kThreads), dim3(kThreads), 0,
+                       stream, t, sorted);
+    return sorted;
+  }
   int range = (t.nrows + 255) / 256;
   if (range > kSortRange) range = kSortRange;
   const dim3 grid((t.nrows + range - 1) / range), block(kSortThreads);
@@ -745,6 +867,7 @@ void sort_tokens(const TokenArg& t, const Sorted& sorted, hipStream_t stream) {
   else
     hipLaunchKernelGGL(sort_tokens_kernel<int64_t>, grid, block, shared, stream, (const int64_t*)t.index,
                        (uint32_t)t.ntokens, t.nrows, range, sorted);
+  return sorted;
 }
 
 // Workgroups of rows_kernel that stay, for the sums over all rows
@@ -757,9 +880,7 @@ hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, voi
   const SortedLayout l = sorted_layout(t.ntokens, t.nrows, t.channels);
   char* base = static_cast<char*>(workspace);
   float* partial = reinterpret_cast<float*>(base + l.partial);
-  const Sorted sorted{reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + l.order),
-                      l.slots ? reinterpret_cast<int32_t*>(base + l.piece_row) : nullptr};
-  sort_tokens(t, sorted, stream);
+  const Sorted sorted = sort_tokens(t, l, base, stream);
   int parts = 0;
   with_packs_of<T>(t.channels, address(grad) | address(out) | address(NORM ? norm.table : nullptr), [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
@@ -785,7 +906,7 @@ hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, voi
     if constexpr (NORM)
       with_team<VEC>(packs, [&](auto shape) { rows(shape, kRowParts, 1); });
     else
-      with_tile<VEC, 4>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
+      with_tile<VEC, MG_K>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
   });
   if (NORM && norm.to_params && parts > 1)
     return launch_sum_partials(norm.norm, norm.params.partial, parts, norm.params.weight, norm.params.bias,

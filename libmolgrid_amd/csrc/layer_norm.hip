@@ -405,6 +405,16 @@ hipError_t sum_partials(const float* partial, int parts, int channels, void* gra
   return hipGetLastError();
 }
 
+// The encoder's rows are bound by arithmetic (the generator alone is half of it), so as many elements
+// a lane as go: what is done once a row (a division and a square root, the sums over the lanes) is
+// then shared by more of them.
+template <int VEC, bool ENCODE, typename F>
+bool with_norm_team(int packs, F f) {
+  if constexpr (ENCODE && VEC == 8)
+    if (packs > 128 && packs <= 256) return f(TeamShape<64, 4>()), true;
+  return with_team<VEC>(packs, f);
+}
+
 template <typename T, bool ENCODE>
 hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x, const void* bias,
                 const DropArg& drop, void* out, float* means, float* rstds, hipStream_t stream) {
@@ -426,7 +436,7 @@ hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x,
   }
   const auto with_packs = [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
-    return with_team<VEC>((a.channels + VEC - 1) / VEC, [&](auto shape) {
+    return with_norm_team<VEC, ENCODE>((a.channels + VEC - 1) / VEC, [&](auto shape) {
       using S = decltype(shape);
       const uint32_t blocks = (nrows + S::TEAMS - 1) / S::TEAMS;
       const uint32_t resident = kResident * 256 / S::THREADS;

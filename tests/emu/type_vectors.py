@@ -71,6 +71,8 @@ def tokens_case(rng):
     channels = drawn_size(rng, max(2, min(1500, 150000 // max(tokens, rows))))
     if rng.random() < 0.5:
         channels = max(8, channels // 8 * 8)
+    if rng.random() < 0.08:                                        # sorted by digits
+        tokens, rows, channels = int(rng.integers(32769, 45000)), drawn_size(rng, 3000) + 32, int(rng.integers(1, 5))
     dtype, kind = TYPES[rng.integers(3)], KINDS[rng.integers(3)]
     t = rng.integers(0, rows, tokens)
     how = rng.integers(4)

@@ -105,6 +105,32 @@ def test_gradient_of_the_table_for_unusual_orders(mg, case, tokens):
     check(got, dw, d_dw, F32, case)
 
 
+@pytest.mark.parametrize("case", ["one row", "nothing", "even", "uneven", "sorted"])
+@pytest.mark.parametrize("tokens,rows", [(32768, 700), (32769, 33), (33000, 511), (40960, 512), (50001, 5000),
+                                         (36000, 300000)])
+def test_gradient_of_the_table_for_many_tokens(mg, case, tokens, rows):
+    """On either side of where the tokens are sorted by digits: one, two and three digits, whole and
+    broken tiles, tokens without a row."""
+    channels = 3
+    rng = np.random.default_rng(tokens)
+    index = {"one row": np.full(tokens, rows - 1), "nothing": np.full(tokens, -1),
+             "even": rng.integers(0, rows, tokens),
+             "uneven": np.minimum(rng.integers(0, rows, tokens), rng.integers(0, rows, tokens) // 50),
+             "sorted": np.sort(rng.integers(0, rows, tokens))}[case]
+    index[rng.random(tokens) < 0.1] = rows                        # names no row
+    grad = values(rng, (tokens, channels), F32)
+    (dw, d_dw), _ = ref.embed_backward(np.where(index < rows, index, -1), f64(grad), np.zeros((rows, channels)), 1.0)
+    index, table = torch.tensor(index).cuda(), torch.zeros((rows, channels)).cuda()
+    got, _ = mg.embed_types_backward(grad.cuda(), index, table)
+    check(got, dw, d_dw, F32, case)
+    weight = torch.ones(channels).cuda()
+    to = mg.encode_types_backward(grad.cuda(), index, table + 1, weight, p=0.5, seed=3)
+    at = np.where(index.cpu().numpy() < rows, index.cpu().numpy(), -1)
+    for g, expected in zip(to, ref.encode_backward(at, f64(grad), np.ones((rows, channels)), 1.0, np.ones(channels),
+                                                   1e-5, 0.5, 3, 0)):
+        check(g, *expected, F32, case)
+
+
 def test_indices_that_name_no_row(mg):
     """Not-a-number, infinities, numbers beyond 32 bits and between the rows; infinities and
     not-a-number in the gradients of tokens without a row stay out of the sums."""
