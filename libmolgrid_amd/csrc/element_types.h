@@ -119,17 +119,6 @@ template <typename T, int VEC>
 __device__ __forceinline__ void store_floats(T* p, const float (&in)[VEC]) {
   Pack<T, VEC> pack;
   pack.set(in);
-#ifdef MG_NT
-  if constexpr (sizeof(T) * VEC >= 16) {
-    typedef uint32_t Four __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int i = 0; i < Pack<T, VEC>::kWords; i += 4) {
-      const Four v = {pack.w[i], pack.w[i + 1], pack.w[i + 2], pack.w[i + 3]};
-      __builtin_nontemporal_store(v, reinterpret_cast<Four*>(p) + i / 4);
-    }
-    return;
-  } else
-#endif
   *reinterpret_cast<Pack<T, VEC>*>(p) = pack;
 }
 

@@ -14,22 +14,55 @@
 #include "kernels.h"
 #include "row_team.h"
 
-#ifndef MG_K
-#define MG_K 4
-#endif
 namespace mg {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kResident = 2048;   // workgroups of 256 threads that fill the chip
 
-// A team takes one token at a time; the index of its next token is read ahead.
+// Rows that a team of LANES lanes holds with a pack each: it takes kTokens tokens at a time, whose
+// indices, and then rows, are loaded together.
+constexpr int kTokens = 4;
+
 template <typename T, int VEC, int LANES>
+__global__ __launch_bounds__(kThreads) void embed_narrow_kernel(TokenArg t, const T* __restrict__ table,
+                                                                float scale,
+                                                                const float* __restrict__ scales,
+                                                                T* __restrict__ out) {
+  constexpr int kTeams = kThreads / LANES;
+  const int c = threadIdx.x % LANES * VEC, team = threadIdx.x / LANES;
+  const uint32_t ntokens = (uint32_t)t.ntokens;
+  for (uint32_t n0 = blockIdx.x * kTeams * kTokens; n0 < ntokens; n0 += gridDim.x * kTeams * kTokens) {
+    uint32_t n[kTokens];
+    int row[kTokens];
+    float by[kTokens], v[kTokens][VEC];
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) n[u] = n0 + u * kTeams + team;
+    token_rows(t, n, ntokens, row);
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      by[u] = scales ? scales[n[u] < ntokens ? n[u] : 0] : scale;
+      if (t.nrows > 0)
+        load_floats<T, VEC>(table + (size_t)(row[u] < 0 ? 0 : row[u]) * t.channels + (c < t.channels ? c : 0), v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      if (n[u] >= ntokens || c >= t.channels) continue;
+      // (a row that is not there is zero whatever the scale is)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[u][i] = row[u] < 0 ? 0.f : by[u] * v[u][i];
+      store_floats<T, VEC>(out + (size_t)n[u] * t.channels + c, v[u]);
+    }
+  }
+}
+
+// Wider rows: a wave takes one token at a time; the index of its next token is read ahead.
+template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void embed_kernel(TokenArg t, const T* __restrict__ table,
                                                          float scale,
                                                          const float* __restrict__ scales,
                                                          T* __restrict__ out) {
-  constexpr int kTeams = kThreads / LANES, kUnroll = 4;
+  constexpr int LANES = kWave, kTeams = kThreads / LANES, kUnroll = 4;
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const uint32_t step = gridDim.x * kTeams, ntokens = (uint32_t)t.ntokens;
   uint32_t n = blockIdx.x * kTeams + team;
@@ -56,7 +89,6 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(TokenArg t, const T* __
       for (int u = 0; u < kUnroll; ++u) {
         const int c = c0 + u * LANES * VEC;
         if (c >= t.channels) break;
-        // (a row that is not there is zero whatever the scale is)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[u][i] = at < 0 ? 0.f : by * v[u][i];
         store_floats<T, VEC>(to + c, v[u]);
@@ -156,6 +188,7 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T*
   for (int i = 0; i < t.nrows * VEC; ++i) mine[i * LANES] = 0.f;
   if (SCALES) {
     float* to = copies + teams * copy;
+#pragma unroll 8
     for (int i = threadIdx.x; i < copy; i += blockDim.x) {
       const int at = i % LANES * VEC + i / LANES % VEC;
       to[i] = at < t.channels ? widen(table[(size_t)(i / (LANES * VEC)) * t.channels + at]) : 0.f;
@@ -195,6 +228,7 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T*
   __syncthreads();
   for (int i = threadIdx.x; i < copy; i += blockDim.x) {
     float sum = 0.f;
+#pragma unroll 16
     for (int k = 0; k < teams; ++k) sum += copies[k * copy + i];
     const int at = blockIdx.y * LANES * VEC + (i % LANES) * VEC + i / LANES % VEC;
     if (at >= t.channels) continue;
@@ -218,10 +252,7 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
   const size_t e = (size_t)blockIdx.x * kWave + lane;
   const int share = (parts + kSumWaves - 1) / kSumWaves;
   const int end = min(parts, (wave + 1) * share);
-  float sum = 0.f;
-  if (e < elements)
-#pragma unroll 16
-    for (int i = wave * share; i < end; ++i) sum += partial[(size_t)i * elements + e];
+  float sum = e < elements ? column_sum(partial, elements, e, wave * share, end) : 0.f;
   sums[wave][lane] = sum;
   lds_barrier();
   if (wave != 0 || e >= elements) return;
@@ -246,7 +277,7 @@ constexpr int kOneLaunchTokens = 32768;
 // starts in and f whether it is its row's first: of a block's positions at most two start pieces, a
 // first one (its row then holds the block's last position) and a later one (its row then holds the
 // block's first position).
-constexpr int kBlock = 16, kDirect = 32;
+constexpr int kBlock = 16, kDirect = 16;
 
 __device__ __forceinline__ int piece_length(int count) {
   return ((int)(0.5f * sqrtf((float)count)) / kBlock + 1) * kBlock;
@@ -701,10 +732,12 @@ unsigned at_most(size_t blocks, size_t most) { return (unsigned)(blocks < most ?
 // The lanes of a team for rows of `packs` packs where wider rows are gone through in steps
 template <int VEC, typename F>
 void with_lanes(int packs, F f) {
-  if (VEC > 1 && packs <= 4) return f(std::integral_constant<int, 4>());
-  if (VEC > 1 && packs <= 8) return f(std::integral_constant<int, 8>());
+  if constexpr (VEC > 1) {
+    if (packs <= 4) return f(std::integral_constant<int, 4>());
+    if (packs <= 8) return f(std::integral_constant<int, 8>());
+    if (packs > 16 && packs <= 32) return f(std::integral_constant<int, 32>());
+  }
   if (packs <= 16) return f(std::integral_constant<int, 16>());
-  if (VEC > 1 && packs <= 32) return f(std::integral_constant<int, 32>());
   return f(std::integral_constant<int, 64>());
 }
 template <typename T, typename F>
@@ -723,8 +756,12 @@ hipError_t embed(const TokenArg& t, const void* table, float scale, const float*
     with_lanes<VEC>(t.channels / VEC, [&](auto lanes) {
       constexpr int LANES = decltype(lanes)::value;
       const size_t blocks = ((size_t)t.ntokens * LANES + kThreads - 1) / kThreads;
-      hipLaunchKernelGGL((embed_kernel<T, VEC, LANES>), dim3(at_most(blocks, kResident)), dim3(kThreads), 0,
-                         stream, t, (const T*)table, scale, scales, (T*)out);
+      if (t.channels <= LANES * VEC)
+        hipLaunchKernelGGL((embed_narrow_kernel<T, VEC, LANES>), dim3(at_most((blocks + kTokens - 1) / kTokens, kResident)),
+                           dim3(kThreads), 0, stream, t, (const T*)table, scale, scales, (T*)out);
+      else
+        hipLaunchKernelGGL((embed_kernel<T, VEC>), dim3(at_most(blocks, kResident)), dim3(kThreads), 0, stream, t,
+                           (const T*)table, scale, scales, (T*)out);
     });
   });
   return hipGetLastError();
@@ -906,7 +943,7 @@ hipError_t sorted_rows(const TokenArg& t, const void* grad, const SumArg& a, voi
     if constexpr (NORM)
       with_team<VEC>(packs, [&](auto shape) { rows(shape, kRowParts, 1); });
     else
-      with_tile<VEC, MG_K>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
+      with_tile<VEC, 4>(packs, [&](auto shape) { rows(shape, kResident, tiles(shape)); });
   });
   if (NORM && norm.to_params && parts > 1)
     return launch_sum_partials(norm.norm, norm.params.partial, parts, norm.params.weight, norm.params.bias,

@@ -138,22 +138,27 @@ __global__ __launch_bounds__(kThreads) void few_rows_encode_kernel(
   HIP_DYNAMIC_SHARED(float, vectors);   // [nrows][channels]
   uint64_t seed, offset;
   drop_key(arg, seed, offset);
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, channels = t.channels;
+  // eight lanes a row: a table of few rows goes through in one round
+  constexpr int LANES = 8, kTeams = kThreads / LANES;
+  const int lane = threadIdx.x % LANES, channels = t.channels;
   const bool is_float = a.param_dtype == MG_FLOAT32;
-  for (int row = wave; row < t.nrows; row += kWaves) {
+  for (int row0 = 0; row0 < t.nrows; row0 += kTeams) {
+    const int row = row0 + threadIdx.x / LANES, count = row < t.nrows ? channels : 0;
     float* v = vectors + row * channels;
     float sum = 0.f, squares = 0.f;
-    for (int c = lane; c < channels; c += kWave) {
+#pragma unroll 4
+    for (int c = lane; c < count; c += LANES) {
       v[c] = scale * widen(table[(size_t)row * channels + c]);
       sum += v[c];
     }
-    const float mean = lanes_sum(sum) / channels;
-    for (int c = lane; c < channels; c += kWave) {   // (every lane its own elements)
+    const float mean = team_sum_in_wave<LANES>(sum) / channels;
+    for (int c = lane; c < count; c += LANES) {   // (every lane its own elements)
       const float d = v[c] - mean;
       squares = fmaf(d, d, squares);
     }
-    const float rstd = 1.f / sqrtf(lanes_sum(squares) / channels + a.eps);
-    for (int c = lane; c < channels; c += kWave)
+    const float rstd = 1.f / sqrtf(team_sum_in_wave<LANES>(squares) / channels + a.eps);
+#pragma unroll 4
+    for (int c = lane; c < count; c += LANES)
       v[c] = fmaf((v[c] - mean) * rstd, param_at<T>(a.weight, is_float, c, 1.f), param_at<T>(bias, is_float, c, 0.f));
   }
   __syncthreads();
@@ -382,10 +387,7 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_partials_kernel(
   const size_t columns = (size_t)2 * channels, c = (size_t)blockIdx.x * kWave + lane;
   const int share = (parts + kSumWaves - 1) / kSumWaves;
   const int end = min(parts, (wave + 1) * share);
-  float sum = 0.f;
-  if (c < columns)
-#pragma unroll 16
-    for (int i = wave * share; i < end; ++i) sum += partial[(size_t)i * columns + c];
+  float sum = c < columns ? column_sum(partial, columns, c, wave * share, end) : 0.f;
   sums[wave][lane] = sum;
   lds_barrier();
   if (wave != 0 || c >= columns) return;

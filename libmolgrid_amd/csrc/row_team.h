@@ -51,13 +51,17 @@ bool with_team(int packs, F f) {
 // Teams of a wave or less for rows that are gone through in tiles of up to `most` packs a lane
 template <int VEC, int MOST, typename F>
 void with_tile(int packs, F f) {
-  if (VEC > 1 && packs <= 4) return f(TeamShape<4, 1>());
-  if (VEC > 1 && packs <= 8) return f(TeamShape<8, 1>());
+  if constexpr (VEC > 1) {
+    if (packs <= 4) return f(TeamShape<4, 1>());
+    if (packs <= 8) return f(TeamShape<8, 1>());
+    if (packs > 16 && packs <= 32) return f(TeamShape<32, 1>());
+  }
   if (packs <= 16) return f(TeamShape<16, 1>());
-  if (VEC > 1 && packs <= 32) return f(TeamShape<32, 1>());
-  if (packs <= 64 || MOST == 1) return f(TeamShape<64, 1>());
-  if (packs <= 128 || MOST == 2) return f(TeamShape<64, 2>());
-  return f(TeamShape<64, 4>());
+  if constexpr (MOST > 1) {
+    if (packs > 64 && packs <= 128) return f(TeamShape<64, 2>());
+    if (packs > 128) return f(TeamShape<64, 4>());
+  }
+  return f(TeamShape<64, 1>());
 }
 
 // Elements of a pack for rows of `channels` elements in arrays whose addresses are ORed together in
@@ -187,15 +191,30 @@ __device__ __forceinline__ void team_stats(float (&v)[K][VEC], int channels, int
   mean = sum[0] / channels;   // (a product could be contracted into the differences)
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const bool inside = (k * LANES + lane) * VEC < channels;
+    if ((k * LANES + lane) * VEC < channels)   // (zeros beyond)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[k][i] = inside ? v[k][i] - mean : 0.f;
-      squares[0] = fmaf(v[k][i], v[k][i], squares[0]);
-    }
+      for (int i = 0; i < VEC; ++i) {
+        v[k][i] -= mean;
+        squares[0] = fmaf(v[k][i], v[k][i], squares[0]);
+      }
   }
   team_sums<LANES>(squares, slots_b);
   rstd = 1.f / sqrtf(squares[0] / channels + eps);
+}
+
+// Column `at` of rows begin .. end - 1 (of `stride` floats) added up, sixteen loads at a time, the last
+// ones too.
+__device__ __forceinline__ float column_sum(const float* rows, size_t stride, size_t at, int begin, int end) {
+  constexpr int U = 16;
+  float sum = 0.f;
+  for (int i0 = begin; i0 < end; i0 += U) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = rows[(size_t)min(i0 + u, end - 1) * stride + at];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += i0 + u < end ? v[u] : 0.f;
+  }
+  return sum;
 }
 
 // Where the sums of a norm's parameter gradients go: as they are if one workgroup has them all,

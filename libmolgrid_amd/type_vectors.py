@@ -75,16 +75,16 @@ def _tensor(x, name, dtypes):
         x = _gr._unwrap(x)
         if not isinstance(x, torch.Tensor):
             raise ValueError("%s: expected a tensor" % name)
+    if x.dtype in dtypes and x.is_cuda and x.get_device() == torch.cuda.current_device() and x.is_contiguous():
+        return x
     if x.dtype not in dtypes:
         raise ValueError("%s: %s is not supported here" % (name, x.dtype))
     if not x.is_cuda:
         raise ValueError("%s: tensor is on the host, others are on the device" % name)
-    if x.device.index != torch.cuda.current_device():
+    if x.get_device() != torch.cuda.current_device():
         raise ValueError("%s: tensor is on device %d but the current device is %d"
-                         % (name, x.device.index, torch.cuda.current_device()))
-    if not x.is_contiguous():
-        raise ValueError("%s: tensor is not contiguous" % name)
-    return x
+                         % (name, x.get_device(), torch.cuda.current_device()))
+    raise ValueError("%s: tensor is not contiguous" % name)
 
 
 def _ptr(x):
