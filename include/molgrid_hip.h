@@ -337,7 +337,7 @@ int mg_widen(const float* src, double* dst, size_t n, void* stream);
  * number below it, as in mg_forward_index; an index below 0, at or beyond nrows,
  * or not-a-number names no row.  Array pointers are aligned to their elements
  * (MG_ERR_INVALID_ARGUMENT otherwise), workspaces to 256 bytes.  Up to 1,048,576
- * channels (MG_ERR_UNSUPPORTED beyond).  Sums over tokens or rows are float, in
+ * channels and fewer than 2^28 tokens and table rows (MG_ERR_UNSUPPORTED beyond).  Sums over tokens or rows are float, in
  * an order that the sizes, the indices and the arrays' alignment alone decide:
  * the same call gives the same bits. */
 enum { MG_FLOAT32 = 0, MG_FLOAT16 = 1, MG_BFLOAT16 = 2 };
@@ -404,7 +404,8 @@ int mg_encode_types(int ntokens, int nrows, int channels, int dtype, int param_d
 /* Gradients of mg_encode_types: grad_table [nrows, channels], grad_weight and
  * grad_bias [channels]; each may be NULL.  All tokens of a row share its
  * normed vector and the norm's backward pass is linear in the gradient, so the
- * gradients of a row's tokens are summed first. */
+ * gradients of a row's tokens are summed first.  Rows that no token names have
+ * no part in any of the gradients, whatever stands in them. */
 size_t mg_encode_types_backward_workspace_size(int ntokens, int nrows, int channels);
 int mg_encode_types_backward(int ntokens, int nrows, int channels, int dtype, int param_dtype,
                              int index_kind, const void* type_index, const void* grad,

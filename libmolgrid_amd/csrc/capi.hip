@@ -88,10 +88,12 @@ size_t dtype_size(int dtype) { return dtype == MG_FLOAT32 ? 4 : 2; }
 size_t index_size(int kind) { return kind == MG_INDEX_INT64 ? 8 : 4; }
 
 constexpr int kMaxVectorChannels = 1 << 20;   // (launches have a workgroup for every 64 of them)
+constexpr int kMaxTokens = 1 << 28;           // (a launch has fewer than 2^32 threads)
 
 int check_tokens(const TokenArg& t) {
   if (t.ntokens < 0 || t.nrows < 0 || t.channels < 0) return MG_ERR_INVALID_ARGUMENT;
   if (t.channels > kMaxVectorChannels) return MG_ERR_UNSUPPORTED;
+  if (t.ntokens >= kMaxTokens || t.nrows >= kMaxTokens) return MG_ERR_UNSUPPORTED;
   if (!is_dtype(t.dtype)) return MG_ERR_INVALID_ARGUMENT;
   if (t.index_kind < MG_INDEX_FLOAT32 || t.index_kind > MG_INDEX_INT64) return MG_ERR_INVALID_ARGUMENT;
   if (!aligned(t.index, index_size(t.index_kind))) return MG_ERR_INVALID_ARGUMENT;

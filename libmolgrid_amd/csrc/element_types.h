@@ -34,6 +34,14 @@ struct DropArg {
   uint64_t seed, offset;  // unless state is given
   const uint64_t* state;  // device: {seed, offset}
 };
+// Which rows of a table tokens name: by bits (of up to 32 rows, in `count` words that are ORed
+// together), or by where the sorted tokens of a row begin and end.
+struct NamedRows {
+  const uint32_t* words;
+  int count;
+  const int32_t* start;   // or nullptr
+};
+
 // Arrays of 16-bit types are read and written as their bits; everything is computed in float and
 // rounded once, to the nearest, where it is stored.
 struct Half {

@@ -155,8 +155,10 @@ template <typename T, int VEC, int LANES, bool DROP, bool SCALES>
 __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T* __restrict__ grad,
                                                             SumArg a, int share, const T* __restrict__ table,
                                                             float* __restrict__ grad_scales, T* out,
-                                                            float* partial) {
+                                                            float* partial, uint32_t* __restrict__ named) {
   HIP_DYNAMIC_SHARED(float, copies);
+  __shared__ uint32_t any_named;
+  uint32_t my_named = 0;
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const int teams = blockDim.x / LANES;
   const int copy = t.nrows * VEC * LANES;
@@ -209,6 +211,7 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T*
       for (int i = 0; i < VEC; ++i) g[i] = now.g[u][i];
       if (now.row[u] >= 0 && inside) {
         const int at = now.row[u] * VEC * LANES;
+        my_named |= 1u << now.row[u];
         if (SCALES)
 #pragma unroll
           for (int i = 0; i < VEC; ++i) dot = fmaf(g[i], own[at + i * LANES], dot);
@@ -225,7 +228,13 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T*
       }
     }
   }
+  if (named && threadIdx.x == 0) any_named = 0;
   __syncthreads();
+  if (named) {   // (a bit a row: a table of few rows has no more than a word has bits)
+    atomicOr(&any_named, my_named);
+    __syncthreads();
+    if (threadIdx.x == 0 && blockIdx.y == 0) named[blockIdx.x] = any_named;
+  }
   for (int i = threadIdx.x; i < copy; i += blockDim.x) {
     float sum = 0.f;
 #pragma unroll 16
@@ -325,7 +334,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
   constexpr int kAhead = 8;   // indices of a lane in flight
   const auto fetch = [&](uint32_t n) { return n < end ? table_row(index[n], nrows) : -1; };
   int lower = 0;
-  uint64_t held = 0;   // bit b of lane l: step 64 l + b has a token of this workgroup's rows
+  static_assert(kOneLaunchTokens <= 32 * kSortThreads, "a bit for every step");
+  uint32_t held = 0;   // steps that have a token of this workgroup's rows
   for (uint32_t s0 = 0; s0 < steps; s0 += kAhead) {
     uint32_t row[kAhead];   // (no row: larger than any)
 #pragma unroll
@@ -337,7 +347,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
       const bool inside = r < (uint32_t)rows;
       if (__ballot(inside)) {
         if (inside) atomicAdd(&mine[r], 1);
-        if ((uint32_t)lane == s / 64) held |= (uint64_t)1 << (s % 64);
+        held |= 1u << s;
       }
     }
   }
@@ -388,22 +398,18 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
     }
   };
   constexpr int kTogether = 4;
-  for (uint32_t l = 0; l * 64 < steps; ++l) {
-    uint64_t bits = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)held, (int)l) |
-                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(held >> 32), (int)l) << 32;
-    while (bits) {
-      uint32_t n[kTogether];
-      int row[kTogether];
+  while (held) {
+    uint32_t n[kTogether];
+    int row[kTogether];
 #pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const uint32_t s = bits ? l * 64 + (uint32_t)__builtin_ctzll(bits) : steps;
-        bits &= bits - 1;
-        n[u] = begin + s * kWave + lane;
-        row[u] = s < steps ? fetch(n[u]) : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) place(n[u], row[u]);
+    for (int u = 0; u < kTogether; ++u) {
+      const uint32_t s = held ? (uint32_t)__builtin_ctz(held) : steps;
+      held &= held - 1;
+      n[u] = begin + s * kWave + lane;
+      row[u] = s < steps ? fetch(n[u]) : -1;
     }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) place(n[u], row[u]);
   }
 }
 
@@ -787,6 +793,7 @@ size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // How the few-row kernel shares the tokens out.  It is taken for tables of up to kFewRows rows,
 // where a wave's copies fit the LDS of a workgroup.
 constexpr int kFewRows = 32;
+constexpr int kFewRowsParts = 512;   // two workgroups on each of 256 CUs
 struct FewRowsPlan {
   int waves, share, parts;
 };
@@ -797,19 +804,19 @@ FewRowsPlan few_rows_plan(int ntokens, int nrows, int vec, int lanes, int column
   if (p.waves > kThreads / kWave) p.waves = kThreads / kWave;
   if (p.waves < 1) p.waves = 1;
   const int teams = p.waves * kWave / lanes;
-  // two workgroups on each of 256 CUs, but no fewer than two rounds of loads for each
-  size_t share = ((size_t)ntokens * column_blocks + 511) / 512;
+  // kFewRowsParts workgroups, but no fewer than two rounds of loads for each
+  size_t share = ((size_t)ntokens * column_blocks + kFewRowsParts - 1) / kFewRowsParts;
   const size_t least = (size_t)teams * kTableUnroll * 2;
   if (share < least) share = least;
+  if (share > (size_t)ntokens) share = ntokens;
   p.share = (int)share;
   p.parts = (int)(((size_t)ntokens + share - 1) / share);
   return p;
 }
-// (its partial tables are never more than the 512 workgroups')
 size_t few_rows_bytes(int ntokens, int nrows, int channels) {
   // (the smallest share is that of one team)
   size_t parts = ((size_t)ntokens + 2 * kTableUnroll - 1) / (2 * kTableUnroll);
-  if (parts > 512) parts = 512;
+  if (parts > kFewRowsParts) parts = kFewRowsParts;
   return round_up(parts * nrows * channels * sizeof(float));
 }
 
@@ -832,10 +839,11 @@ SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   return l;
 }
 
-// scales_done: whether the gradients of the scales (if any are wanted) came out as well
+// scales_done: whether the gradients of the scales (if any are wanted) came out as well.  named: where
+// the rows that tokens name are written down, a word of bits for each of the workgroups.
 template <typename T, typename O, bool DROP>
 hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, const void* table, float* grad_scales,
-                    bool* scales_done, void* out, float* partial, hipStream_t stream) {
+                    bool* scales_done, void* out, float* partial, NamedRows* named, hipStream_t stream) {
   with_packs_of<T>(t.channels, address(grad), [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
     with_lanes<VEC>(t.channels / VEC, [&](auto lanes) {
@@ -846,15 +854,17 @@ hipError_t few_rows(const TokenArg& t, const void* grad, const SumArg& a, const 
       const size_t copies = (size_t)p.waves * 256 * t.nrows * VEC;
       const size_t own = (size_t)t.nrows * VEC * LANES * sizeof(float);
       const dim3 grid(p.parts, column_blocks), block(p.waves * kWave);
+      uint32_t* words = named ? const_cast<uint32_t*>(named->words) : nullptr;
+      if (named) named->count = p.parts;
       if (!DROP && grad_scales && column_blocks == 1 && copies + own <= kTableLds) {
         if (scales_done) *scales_done = true;
         hipLaunchKernelGGL((few_rows_kernel<T, VEC, LANES, DROP, !DROP>), grid, block, copies + own, stream, t,
                            (const T*)grad, a, p.share, (const T*)table, grad_scales, direct ? (T*)out : nullptr,
-                           direct ? nullptr : partial);
+                           direct ? nullptr : partial, words);
       } else {
         hipLaunchKernelGGL((few_rows_kernel<T, VEC, LANES, DROP, false>), grid, block, copies, stream, t,
                            (const T*)grad, a, p.share, (const T*)table, grad_scales, direct ? (T*)out : nullptr,
-                           direct ? nullptr : partial);
+                           direct ? nullptr : partial, words);
       }
       if (direct) return;
       const size_t elements = (size_t)t.nrows * t.channels;
@@ -995,7 +1005,8 @@ hipError_t embed_backward(const TokenArg& t, const void* grad, const void* table
   if (grad_table && t.nrows > 0 && t.channels > 0)
     e = t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)
         : t.nrows <= kFewRows
-            ? few_rows<T, T, false>(t, grad, a, table, grad_scales, &scales_done, grad_table, (float*)workspace, stream)
+            ? few_rows<T, T, false>(t, grad, a, table, grad_scales, &scales_done, grad_table, (float*)workspace, nullptr,
+                                    stream)
             : sorted_rows<T, T, false, false>(t, grad, a, grad_table, workspace, TableNorm(), stream);
   if (e != hipSuccess || !grad_scales || t.ntokens == 0 || scales_done) return e;
   return scale_gradient<T>(t, grad, table, grad_scales, stream);
@@ -1018,14 +1029,16 @@ bool sums_in_memory(const TokenArg& t) {
   return t.ntokens == 0 || t.nrows <= kFewRows || t.channels > kMostTeamChannels;
 }
 struct EncodeLayout {
-  size_t params, rest, bytes;   // offsets: partial sums of weight and bias, workspace of the row sums
+  size_t params, named, rest, bytes;   // offsets: partial sums of weight and bias, bits of the rows that
+                                       // tokens name, workspace of the row sums
 };
 EncodeLayout encode_layout(const TokenArg& t) {
   EncodeLayout l;
   l.params = sums_in_memory(t) ? round_up((size_t)t.nrows * t.channels * sizeof(float)) : 0;
-  l.rest = l.params + round_up(sums_in_memory(t)
-                                   ? norm_backward_workspace_bytes(t.nrows, t.channels)
-                                   : (size_t)(t.nrows < kRowParts ? t.nrows : kRowParts) * 2 * t.channels * sizeof(float));
+  l.named = l.params + round_up(sums_in_memory(t)
+                                    ? norm_backward_workspace_bytes(t.nrows, t.channels)
+                                    : (size_t)(t.nrows < kRowParts ? t.nrows : kRowParts) * 2 * t.channels * sizeof(float));
+  l.rest = l.named + (t.nrows <= kFewRows ? kFewRowsParts * sizeof(uint32_t) : 0);
   l.bytes = l.rest + (t.ntokens ? embed_backward_workspace_bytes(t.ntokens, t.nrows, t.channels) : 0);
   return l;
 }
@@ -1042,14 +1055,17 @@ hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad
     return sorted_rows<T, T, true, true>(t, grad, a, grad_table, workspace + l.rest, norm, stream);
   }
   float* sums = reinterpret_cast<float*>(workspace);
+  // which rows tokens name: the others have no part in the gradients, whatever stands in them
+  NamedRows named{reinterpret_cast<uint32_t*>(workspace + l.named), 0, nullptr};
+  if (t.nrows > kFewRows && t.ntokens > 0) named = NamedRows{nullptr, 0, reinterpret_cast<int32_t*>(workspace + l.rest)};
   hipError_t e = t.nrows == 0 ? hipSuccess
                  : t.ntokens == 0 ? zero<float>(sums, (size_t)t.nrows * t.channels, stream)
                  : t.nrows <= kFewRows
                      ? few_rows<T, float, true>(t, grad, a, nullptr, nullptr, nullptr, sums, (float*)(workspace + l.rest),
-                                                stream)
+                                                &named, stream)
                      : sorted_rows<T, float, true, false>(t, grad, a, sums, workspace + l.rest, TableNorm(), stream);
   if (e != hipSuccess) return e;
-  return launch_table_norm_backward(n, sums, table, scale, grad_table, grad_weight, grad_bias, params, stream);
+  return launch_table_norm_backward(n, sums, table, scale, named, grad_table, grad_weight, grad_bias, params, stream);
 }
 }  // namespace
 

@@ -131,9 +131,10 @@ hipError_t launch_norm_backward(const NormArg& a, const void* grad, const void* 
                                 const float* means, const float* rstds, void* grad_x,
                                 void* grad_weight, void* grad_bias, void* workspace,
                                 hipStream_t stream);
-// The same for the rows of a scaled table and a float gradient; the statistics are computed again.
+// The same for the rows of a scaled table and a float gradient; the statistics are computed again, and
+// rows that no token names have no part in it.
 hipError_t launch_table_norm_backward(const NormArg& a, const float* sums, const void* table,
-                                      float scale, void* grad_table, void* grad_weight,
+                                      float scale, const NamedRows& named, void* grad_table, void* grad_weight,
                                       void* grad_bias, void* workspace, hipStream_t stream);
 
 // The partial sums of `parts` workgroups (ParamSums), added up.

@@ -238,6 +238,21 @@ __global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenAr
   }
 }
 
+// The words of NamedRows, ORed by the workgroup.
+__device__ __forceinline__ uint32_t named_word(const NamedRows& named) {
+  __shared__ uint32_t all;
+  if (threadIdx.x == 0) all = 0;
+  __syncthreads();
+  uint32_t mine = 0;
+  for (int i = threadIdx.x; i < named.count; i += blockDim.x) mine |= named.words[i];
+  if (mine) atomicOr(&all, mine);
+  __syncthreads();
+  return all;
+}
+__device__ __forceinline__ bool is_named(const NamedRows& named, uint32_t word, uint32_t n) {
+  return named.start ? named.start[n + 1] > named.start[n] : n < 32 && (word >> n & 1);
+}
+
 // Backward: a team holds the rows of x and of the gradient, writes dx, and a lane adds its share of
 // dw and db up over all rows that its team takes.  G: type of the gradient; TABLE: x is a scaled
 // table, whose statistics are computed here.
@@ -246,8 +261,8 @@ constexpr int kParts = 512, kNarrowParts = 1024;   // workgroups that share the 
 template <typename T, typename G, int VEC, int LANES, int K, bool TABLE>
 __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_kernel(
     const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a,
-    const float* __restrict__ means, const float* __restrict__ rstds, T* __restrict__ grad_x,
-    bool to_params, ParamSums params) {
+    const float* __restrict__ means, const float* __restrict__ rstds, NamedRows named,
+    T* __restrict__ grad_x, bool to_params, ParamSums params) {
   using Shape = TeamShape<LANES, K>;
   __shared__ float slots[4][2 * Shape::WAVES];
   HIP_DYNAMIC_SHARED(float, sums);   // dw and db of a workgroup with several teams
@@ -263,13 +278,17 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
   const float inv = 1.f / channels;
   const uint32_t step = gridDim.x * Shape::TEAMS;
 
+  const uint32_t word = TABLE ? named_word(named) : 0;
+
   RowPacks<T, VEC, K> next_x;
   RowPacks<G, VEC, K> next_g;
   float next_mean = 0.f, next_rstd = 0.f;
+  bool next_named = false;
   const auto fetch = [&](uint32_t n) {
     const bool live = n < nrows;
     const size_t at = live ? (size_t)n * channels : 0;
-    load_row<T, VEC, LANES, K>(x + at, channels, lane, live, next_x);
+    next_named = live && (!TABLE || is_named(named, word, n));
+    load_row<T, VEC, LANES, K>(x + at, channels, lane, next_named, next_x);
     load_row<G, VEC, LANES, K>(grad + at, channels, lane, live, next_g);
     if (!TABLE && live) {
       next_mean = means[n];
@@ -283,6 +302,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
     const RowPacks<T, VEC, K> px = next_x;
     const RowPacks<G, VEC, K> pg = next_g;
     float mean = next_mean, rstd = next_rstd;
+    const bool has_part = next_named;
     fetch(n + step);
     float h[K][VEC];
 #pragma unroll
@@ -303,7 +323,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
         const float q = g * w[k][i];
         both[0] += q;
         both[1] = fmaf(q, h[k][i], both[1]);
-        if (n < nrows) dw[k][i] = fmaf(g, h[k][i], dw[k][i]);
+        if (has_part) dw[k][i] = fmaf(g, h[k][i], dw[k][i]);
         db[k][i] += g;
       }
     team_sums<LANES>(both, slots[parity]);
@@ -318,7 +338,7 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float q = pg.pack[k][i] * w[k][i];
-        d[i] = factor * (q - mean_q - h[k][i] * mean_qh);
+        d[i] = has_part ? factor * (q - mean_q - h[k][i] * mean_qh) : 0.f;
       }
       store_floats<T, VEC>(grad_x + (size_t)n * channels + c, d);
     }
@@ -330,12 +350,17 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
 template <typename T, typename G>
 __global__ __launch_bounds__(kThreads) void wide_norm_backward_kernel(
     const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a, const float* means,
-    const float* rstds, T* __restrict__ grad_x) {
+    const float* rstds, NamedRows named, T* __restrict__ grad_x) {
   __shared__ float slots[2][kWaves];
   __shared__ float both_slots[2 * kWaves];
   const bool is_float = a.param_dtype == MG_FLOAT32;
-  for (int n = blockIdx.x; n < a.nrows; n += gridDim.x) {
+  const uint32_t word = means ? 0 : named_word(named);
+  for (uint32_t n = blockIdx.x; n < (uint32_t)a.nrows; n += gridDim.x) {
     const size_t at = (size_t)n * a.channels;
+    if (!means && !is_named(named, word, n)) {
+      for (int c = threadIdx.x; c < a.channels; c += kThreads) grad_x[at + c] = narrow<T>(0.f);
+      continue;
+    }
     const Stats s = means ? Stats{means[n], rstds[n]}
                           : wide_row_stats(x + at, a.channels, scale, a.eps, slots);
     float both[2] = {0.f, 0.f};
@@ -358,12 +383,14 @@ __global__ __launch_bounds__(kThreads) void wide_norm_backward_kernel(
 template <typename T, typename G>
 __global__ __launch_bounds__(kThreads) void wide_norm_params_kernel(
     const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a, const float* means,
-    const float* rstds, float* __restrict__ partial) {
+    const float* rstds, NamedRows named, float* __restrict__ partial) {
   __shared__ float slots[2][kWaves];
   float* row = partial + (size_t)blockIdx.x * 2 * a.channels;
   for (int c = threadIdx.x; c < a.channels; c += kThreads) row[c] = row[a.channels + c] = 0.f;
-  for (int n = blockIdx.x; n < a.nrows; n += gridDim.x) {
+  const uint32_t word = means ? 0 : named_word(named);
+  for (uint32_t n = blockIdx.x; n < (uint32_t)a.nrows; n += gridDim.x) {
     const size_t at = (size_t)n * a.channels;
+    if (!means && !is_named(named, word, n)) continue;
     const Stats s = means ? Stats{means[n], rstds[n]}
                           : wide_row_stats(x + at, a.channels, scale, a.eps, slots);
     for (int c = threadIdx.x; c < a.channels; c += kThreads) {   // (the same thread all along)
@@ -467,8 +494,8 @@ int norm_parts(int nrows, int teams) {
 
 template <typename T, typename G, bool TABLE>
 hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, float scale,
-                         const float* means, const float* rstds, void* grad_x, void* grad_weight,
-                         void* grad_bias, void* workspace, hipStream_t stream) {
+                         const float* means, const float* rstds, const NamedRows& named, void* grad_x,
+                         void* grad_weight, void* grad_bias, void* workspace, hipStream_t stream) {
   const bool to_params = grad_weight || grad_bias;
   float* partial = to_params ? static_cast<float*>(workspace) : nullptr;
   const ParamSums params{partial, grad_weight, grad_bias, a.param_dtype == MG_FLOAT32};
@@ -483,7 +510,7 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
         const size_t shared = S::LANES <= kWave ? (size_t)2 * a.channels * sizeof(float) : 0;
         hipLaunchKernelGGL((norm_backward_kernel<T, G, VEC, S::LANES, S::K, TABLE>), dim3(parts),
                            dim3(S::THREADS), shared, stream, (const G*)grad, (const T*)x, scale, a,
-                           means, rstds, (T*)grad_x, to_params, params);
+                           means, rstds, named, (T*)grad_x, to_params, params);
       });
     };
     const bool whole = whole_packs<T>(a.channels, address(x) | address(grad) | address(grad_x));
@@ -494,10 +521,10 @@ hipError_t norm_backward(const NormArg& a, const void* grad, const void* x, floa
       if (grad_x)
         hipLaunchKernelGGL((wide_norm_backward_kernel<T, G>), dim3(a.nrows < 4096 ? a.nrows : 4096),
                            dim3(kThreads), 0, stream, (const G*)grad, (const T*)x, scale, a, means,
-                           rstds, (T*)grad_x);
+                           rstds, named, (T*)grad_x);
       if (partial)
         hipLaunchKernelGGL((wide_norm_params_kernel<T, G>), dim3(parts), dim3(kThreads), 0, stream,
-                           (const G*)grad, (const T*)x, scale, a, means, rstds, partial);
+                           (const G*)grad, (const T*)x, scale, a, means, rstds, named, partial);
     }
   }
   if (to_params && !(done && parts == 1))
@@ -548,17 +575,17 @@ hipError_t launch_norm_backward(const NormArg& a, const void* grad, const void* 
                                 void* grad_weight, void* grad_bias, void* workspace,
                                 hipStream_t stream) {
 #define MG_CALL(T)                                                                              \
-  norm_backward<T, T, false>(a, grad, x, 1.f, means, rstds, grad_x, grad_weight, grad_bias, workspace, \
+  norm_backward<T, T, false>(a, grad, x, 1.f, means, rstds, NamedRows(), grad_x, grad_weight, grad_bias, workspace, \
                              stream)
   MG_FOR_TYPE(a.dtype, MG_CALL);
 #undef MG_CALL
 }
 
 hipError_t launch_table_norm_backward(const NormArg& a, const float* sums, const void* table,
-                                      float scale, void* grad_table, void* grad_weight,
+                                      float scale, const NamedRows& named, void* grad_table, void* grad_weight,
                                       void* grad_bias, void* workspace, hipStream_t stream) {
 #define MG_CALL(T)                                                                            \
-  norm_backward<T, float, true>(a, sums, table, scale, nullptr, nullptr, grad_table, grad_weight,    \
+  norm_backward<T, float, true>(a, sums, table, scale, nullptr, nullptr, named, grad_table, grad_weight, \
                                 grad_bias, workspace, stream)
   MG_FOR_TYPE(a.dtype, MG_CALL);
 #undef MG_CALL

@@ -118,7 +118,7 @@ def _table_args(type_index, table):
 
 def _scale_args(scale, index):
     """(number, per-token tensor or None)"""
-    if _is_array(scale) and scale.ndim > 0:
+    if _is_array(scale):
         scale = _tensor(scale, "scale", (torch.float32,))
         if scale.shape != index.shape:
             raise ValueError("scale: expected the shape of type_index, %s, got %s"
@@ -143,6 +143,12 @@ def _like(grad, name, shape, dtype):
     if tuple(grad.shape) != tuple(shape):
         raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(grad.shape)))
     return grad
+
+
+def _number(x, name):
+    if _is_array(x):
+        raise ValueError("%s: expected a number" % name)
+    return float(x)
 
 
 def _eps(eps):
@@ -284,7 +290,7 @@ def encode_types(type_index, table, weight=None, bias=None, scale=1.0, eps=1e-5,
     _capi.check(_capi.lib.mg_encode_types(
         n, rows, channels, _DTYPES[table.dtype],
         _DTYPES[params.dtype if params is not None else torch.float32], _INDICES[index.dtype],
-        _ptr(index), _ptr(table), float(scale), _ptr(weight), _ptr(bias), _eps(eps), p, seed, offset,
+        _ptr(index), _ptr(table), _number(scale, "scale"), _ptr(weight), _ptr(bias), _eps(eps), p, seed, offset,
         state_ptr, _ptr(out), _gr._stream()), "encode_types")
     return out
 
@@ -306,7 +312,7 @@ def encode_types_backward(grad, type_index, table, weight=None, scale=1.0, eps=1
     workspace = _workspace(size, table)
     _capi.check(_capi.lib.mg_encode_types_backward(
         n, rows, channels, _DTYPES[table.dtype], _DTYPES[params], _INDICES[index.dtype], _ptr(index),
-        _ptr(grad), _ptr(table), float(scale), _ptr(weight), _eps(eps), p, seed, offset, state_ptr,
+        _ptr(grad), _ptr(table), _number(scale, "scale"), _ptr(weight), _eps(eps), p, seed, offset, state_ptr,
         _ptr(to_table), _ptr(to_weight), _ptr(to_bias), _ptr(workspace), size, _gr._stream()),
         "encode_types_backward")
     return to_table, to_weight, to_bias
@@ -320,7 +326,7 @@ class TypeEmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, type_index, table, scale):
-        per_token = _is_array(scale) and scale.ndim > 0
+        per_token = _is_array(scale)
         ctx.save_for_backward(type_index, table, scale if per_token else None)
         ctx.scale = None if per_token else float(scale)
         return embed_types(type_index, table, scale)

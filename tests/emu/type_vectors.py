@@ -131,6 +131,9 @@ def norm(rng):
     check(back(out, dtype), *n.forward(f64(weight), f64(bias)), dtype, "normed")
     check(back(mean, torch.float32), n.mean[:, 0], n.d_mean[:, 0], torch.float32, "mean")
     check(back(rstd, torch.float32), n.rstd[:, 0], n.d_rstd[:, 0], torch.float32, "rstd")
+    over = put(x)                                                  # in place
+    ok(e.lib.mg_layer_norm(*head, e.ptr(over), e.ptr(a_weight), e.ptr(a_bias), 1e-5, e.ptr(over), None, None, None))
+    assert np.array_equal(over, out)
     to_x = place((rows, channels), dtype)
     to_weight, to_bias = (place((channels,), param) for _ in range(2))
     w, size = workspace(e.lib.mg_layer_norm_backward_workspace_size(rows, channels))

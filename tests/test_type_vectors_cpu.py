@@ -105,6 +105,8 @@ def test_entry_points_refuse_before_they_launch():
     for bad in (dict(index=None), dict(table=None), dict(out=None)):
         assert embed(**bad) == null, bad
     assert embed(n=0, index=None, out=None) == 0 and embed(c=0, table=None) == 0
+    for bad in (dict(n=1 << 28), dict(v=1 << 28), dict(c=(1 << 20) + 1)):
+        assert embed(**bad) == _capi.MG_ERR_UNSUPPORTED, bad
 
     def embed_back(n=3, v=4, c=5, dtype=0, kind=0, index=a, grad=a, table=a, scales=None, to_table=a,
                    to_scales=None, workspace=a, size=1 << 30):

@@ -334,6 +334,27 @@ def test_encoding(mg, shape, rows, channels, dtype, param, kind, p, shifted):
     assert torch.equal(mg.encode_types_backward(d_grad, d_index, d_table, d_weight, **numbers, state=state)[0], to[0])
 
 
+@pytest.mark.parametrize("rows,channels", [(6, 8), (6, 300), (6, 9001), (60, 8), (60, 300), (40, 9001)])
+@pytest.mark.parametrize("tokens", [0, 3, 500])
+def test_rows_without_tokens_have_no_part(mg, rows, channels, tokens):
+    """Infinities, not-a-number and rows without spread (eps 0) in rows that no token names: zeros in
+    their own gradient, nothing in the others'."""
+    rng = np.random.default_rng(rows + channels)
+    index = torch.tensor(rng.integers(0, 3, tokens))
+    table, grad = values(rng, (rows, channels), F32), values(rng, (tokens, channels), F32)
+    weight = values(rng, channels, F32, 0.2, 1.0)
+    args = (1.5, f64(weight), 0.0, 0.25, 7, 8)
+    expected = ref.encode_backward(index.numpy(), f64(grad), f64(table[:3]), *args)
+    table[3], table[4], table[5:] = math.nan, math.inf, 0.5
+    got = mg.encode_types_backward(grad.cuda(), index.cuda(), table.cuda(), weight.cuda(), scale=1.5, eps=0.0,
+                                   p=0.25, seed=7, offset=8)
+    assert not got[0][3:].any()
+    for g, (value, bound) in zip((got[0][:3], got[1], got[2]), expected):
+        check(g, value, bound, F32)
+    y = mg.encode_types(index.cuda(), table.cuda(), weight.cuda(), scale=1.5, eps=0.0)
+    assert torch.isfinite(y).all()
+
+
 def test_encoding_is_its_parts_one_after_the_other(mg):
     """float32, where the parts round nothing away: within the bounds of the one pass, twice."""
     rng = np.random.default_rng(8)
@@ -508,6 +529,9 @@ def test_refusals(mg):
         lambda: mg.embed_types(t.double(), w), lambda: mg.embed_types(t, w.double()),
         lambda: mg.embed_types(t, w[0]), lambda: mg.embed_types(t, w.t()), lambda: mg.embed_types(t, w.cpu()),
         lambda: mg.embed_types(t, w, torch.ones(3).cuda()), lambda: mg.embed_types(t, w, torch.ones(4).double().cuda()),
+        lambda: mg.embed_types(t, w, torch.tensor(2.0).cuda()), lambda: mg.embed_types(t, w, torch.ones((4, 1)).cuda()),
+        lambda: mg.encode_types(t, w, scale=torch.ones(4).cuda()),
+        lambda: mg.encode_types_backward(x, t, w, scale=torch.tensor(1.0).cuda()),
         lambda: mg.embed_types_backward(x.half(), t, w), lambda: mg.embed_types_backward(x[:3], t, w),
         lambda: mg.embed_types_backward(x[:, ::2], t, w),
         lambda: mg.layer_norm(x, m), lambda: mg.layer_norm(x, w[0].half()), lambda: mg.layer_norm(x.double()),
