@@ -88,7 +88,7 @@ def _tensor(x, name, dtypes):
 
 
 def _ptr(x):
-    return x.data_ptr() if x is not None and x.numel() else None
+    return None if x is None else x.data_ptr()
 
 
 def _empty(shape, like, dtype=None):
@@ -99,6 +99,12 @@ def _workspace(size, like):
     """Device memory of one call: the allocator hands it to later work of this stream only, and a
     captured graph's calls get theirs from that graph's pool."""
     return like.new_empty(size, dtype=torch.uint8) if size else None
+
+
+# bytes of workspace by sizes (a call into the library costs as much as four tensor attributes)
+@functools.lru_cache(maxsize=256)
+def _workspace_size(entry, *sizes):
+    return getattr(_capi.lib, entry + "_workspace_size")(*sizes)
 
 
 def _count(n, name):
@@ -131,16 +137,21 @@ def _param(x, name, channels, dtype, like=None):
     if x is None:
         return None
     _tensor(x, name, _DTYPES)
-    if tuple(x.shape) != (channels,):
+    if x.shape != (channels,):
         raise ValueError("%s: expected shape (%d,), got %s" % (name, channels, tuple(x.shape)))
     if x.dtype not in (torch.float32, dtype) or (like is not None and x.dtype != like.dtype):
         raise ValueError("%s: parameters are float32 or of the vectors' type, and alike" % name)
     return x
 
 
+def _param_gradients(weight, channels, like):
+    first = torch.empty_like(weight) if weight is not None else _empty((channels,), like, torch.float32)
+    return first, torch.empty_like(first)
+
+
 def _like(grad, name, shape, dtype):
     _tensor(grad, name, (dtype,))
-    if tuple(grad.shape) != tuple(shape):
+    if grad.shape != shape:
         raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(grad.shape)))
     return grad
 
@@ -200,7 +211,7 @@ def embed_types_backward(grad, type_index, table, scale=1.0, table_gradient=True
     to_table = torch.empty_like(table) if table_gradient else None
     to_scale = _empty(index.shape, table, torch.float32) if scale_gradient and scales is not None \
         else None
-    size = _capi.lib.mg_embed_types_backward_workspace_size(n, rows, channels) if table_gradient else 0
+    size = _workspace_size("mg_embed_types_backward", n, rows, channels) if table_gradient else 0
     workspace = _workspace(size, table)
     _capi.check(_capi.lib.mg_embed_types_backward(
         n, rows, channels, _DTYPES[table.dtype], _INDICES[index.dtype], _ptr(index), _ptr(grad),
@@ -226,7 +237,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     bias = _param(bias, "bias", channels, x.dtype, weight)
     params = weight if weight is not None else bias
     out = torch.empty_like(x)
-    mean, rstd = _empty((2,) + x.shape[:-1], x, torch.float32).unbind()
+    mean = _empty(x.shape[:-1], x, torch.float32)
+    rstd = torch.empty_like(mean)
     if channels == 0:
         mean.zero_(), rstd.zero_()
     _capi.check(_capi.lib.mg_layer_norm(
@@ -244,14 +256,14 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, input_gradient=True,
     None."""
     x, rows, channels = _norm_sizes(x)
     grad = _like(grad, "grad", x.shape, x.dtype)
-    mean = _like(mean, "mean", x.shape[:-1], torch.float32)
-    rstd = _like(rstd, "rstd", x.shape[:-1], torch.float32)
+    rows_shape = x.shape[:-1]
+    mean = _like(mean, "mean", rows_shape, torch.float32)
+    rstd = _like(rstd, "rstd", rows_shape, torch.float32)
     weight = _param(weight, "weight", channels, x.dtype)
     params = weight.dtype if weight is not None else torch.float32
     to_x = torch.empty_like(x) if input_gradient else None
-    to_weight, to_bias = (_empty((2, channels), x, params).unbind() if param_gradients
-                          else (None, None))
-    size = _capi.lib.mg_layer_norm_backward_workspace_size(rows, channels) if param_gradients else 0
+    to_weight, to_bias = _param_gradients(weight, channels, x) if param_gradients else (None, None)
+    size = _workspace_size("mg_layer_norm_backward", rows, channels) if param_gradients else 0
     workspace = _workspace(size, x)
     _capi.check(_capi.lib.mg_layer_norm_backward(
         rows, channels, _DTYPES[x.dtype], _DTYPES[params], _ptr(grad), _ptr(x), _ptr(mean),
@@ -306,9 +318,8 @@ def encode_types_backward(grad, type_index, table, weight=None, scale=1.0, eps=1
     params = weight.dtype if weight is not None else torch.float32
     p, seed, offset, state_ptr = _drop_args(p, seed, offset, state)
     to_table = torch.empty_like(table) if table_gradient else None
-    to_weight, to_bias = (_empty((2, channels), table, params).unbind() if param_gradients
-                          else (None, None))
-    size = _capi.lib.mg_encode_types_backward_workspace_size(n, rows, channels)
+    to_weight, to_bias = _param_gradients(weight, channels, table) if param_gradients else (None, None)
+    size = _workspace_size("mg_encode_types_backward", n, rows, channels)
     workspace = _workspace(size, table)
     _capi.check(_capi.lib.mg_encode_types_backward(
         n, rows, channels, _DTYPES[table.dtype], _DTYPES[params], _INDICES[index.dtype], _ptr(index),
