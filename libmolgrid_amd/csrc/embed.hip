@@ -21,7 +21,8 @@ constexpr int kThreads = 256;
 constexpr int kResident = 2048;   // workgroups of 256 threads that fill the chip
 
 // Rows that a team of LANES lanes holds with a pack each: it takes kTokens tokens at a time, whose
-// indices, and then rows, are loaded together.
+// indices, and then rows, are loaded together.  204,000 tokens of 28 channels of float: 8.3 us (23 MB
+// written); the waits for index and row are what is left.
 constexpr int kTokens = 4;
 
 template <typename T, int VEC, int LANES>
@@ -56,7 +57,9 @@ __global__ __launch_bounds__(kThreads) void embed_narrow_kernel(TokenArg t, cons
   }
 }
 
-// Wider rows: a wave takes one token at a time; the index of its next token is read ahead.
+// Wider rows: a wave takes one token at a time; the index of its next token is read ahead.  Memory
+// bound: 65,536 tokens of 4,096 channels of bfloat16 in 153 us (0.54 GB written, 0.16 GB of rows read
+// at least once: 4.6 TB/s).
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void embed_kernel(TokenArg t, const T* __restrict__ table,
                                                          float scale,
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(TokenArg t, const T* __
   }
 }
 
-// ds: a team takes one token at a time.
+// ds: a team takes one token at a time.  Where a small table's gradient is summed, ds comes out there.
 template <typename T, int VEC, int LANES>
 __global__ __launch_bounds__(kThreads) void scale_gradient_kernel(TokenArg t,
                                                                   const T* __restrict__ grad,
@@ -149,7 +152,8 @@ constexpr int kTableUnroll = 8;       // tokens of a team in flight
 
 //
 // The tokens of a team go through in rounds of kTableUnroll, a round's loads in flight while the
-// round before it is added.  SCALES: the gradients of the tokens' scales come out on the way
+// round before it is added: 204,000 tokens, 28 rows of 28 floats with SCALES in 18.3 us, 121,250 of 32
+// floats with DROP in 14 us, and 4 us for the second launch.  SCALES: the gradients of the tokens' scales come out on the way
 // (one tile of channels then holds a row), with the table itself in LDS behind the copies.
 template <typename T, int VEC, int LANES, bool DROP, bool SCALES>
 __global__ __launch_bounds__(kThreads) void few_rows_kernel(TokenArg t, const T* __restrict__ grad,
@@ -277,6 +281,8 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
 // 16 us for 16,384, 45 us for 65,536 and 181 us for 262,144 of a vocabulary (131,072 rows).  More
 // tokens are sorted by digits of their row, two launches for each of 9 bits, whose time hardly depends
 // on the tokens.  Both give the same order: rows ascending, and the tokens of a row as they were.
+// (Table gradients of eight floats a row, one launch and digits: 27 and 45 us for 12,000 tokens, 44 and
+// 51 us for 32,768.)
 constexpr int kOneLaunchTokens = 32768;
 
 // A row of up to kDirect tokens is added up by one team.  Longer ones are cut into pieces that
@@ -621,7 +627,9 @@ struct TableNorm {
 };
 
 // Every row of the table: the sum of its tokens, or of its pieces; tiles of channels along the
-// grid's y.  What the next rows need is read ahead: their bounds two rows, their first tokens one.
+// grid's y.  65,536 tokens into 131,072 rows of 4,096 bfloat16: 273 us (1.07 GB written, 0.27 GB read:
+// 4.9 TB/s), and 70 us for the pieces (0.27 GB); with NORM, 32,768 tokens into 32,000 rows of 2,048:
+// 79 and 30 us, bound by the waits of one row after the other and the generator.  What the next rows need is read ahead: their bounds two rows, their first tokens one.
 // NORM: the sum is the gradient of the row's normed vector, which is taken back through the norm
 // while it is here (a team then holds the whole row); the workgroups stay, and their teams' shares
 // of the gradients of weight and bias are added up at the end.
@@ -790,8 +798,8 @@ hipError_t scale_gradient(const TokenArg& t, const void* grad, const void* table
 
 size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// How the few-row kernel shares the tokens out.  It is taken for tables of up to kFewRows rows,
-// where a wave's copies fit the LDS of a workgroup.
+// How the few-row kernel shares the tokens out.  It is for tables of up to kFewRows rows, where a
+// wave's copies fit the LDS of a workgroup.
 constexpr int kFewRows = 32;
 constexpr int kFewRowsParts = 512;   // two workgroups on each of 256 CUs
 struct FewRowsPlan {
@@ -818,6 +826,27 @@ size_t few_rows_bytes(int ntokens, int nrows, int channels) {
   size_t parts = ((size_t)ntokens + 2 * kTableUnroll - 1) / (2 * kTableUnroll);
   if (parts > kFewRowsParts) parts = kFewRowsParts;
   return round_up(parts * nrows * channels * sizeof(float));
+}
+
+// Whether the copies are the better way: where the workgroups' tables, which are written and read
+// again, are no more than two thirds of the gradient, or a single one is enough.  Sums alone, copies
+// and sorted: 204,000 tokens, 28 rows of 28 floats 17 and 56 us, 30,000 x 28 x 256 floats 28 and 45
+// us, 2,000 x 28 x 32 bfloat16 14 and 15 us; but 2,000 x 28 x 256 floats 21 and 15 us, 20,000 x 32 x
+// 512 bfloat16 66 and 33 us, 2,000 x 28 x 2,048 bfloat16 57 and 16 us.
+template <typename T>
+bool copies_pay(const TokenArg& t, const void* grad) {
+  if (t.nrows > kFewRows) return false;
+  bool pay = false;
+  with_packs_of<T>(t.channels, address(grad), [&](auto vec) {
+    constexpr int VEC = decltype(vec)::value;
+    with_lanes<VEC>(t.channels / VEC, [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value;
+      const FewRowsPlan p = few_rows_plan(t.ntokens, t.nrows, VEC, LANES,
+                                          (t.channels + LANES * VEC - 1) / (LANES * VEC));
+      pay = p.parts == 1 || (size_t)3 * t.nrows * sizeof(float) <= (size_t)2 * p.share * sizeof(T);
+    });
+  });
+  return pay;
 }
 
 struct SortedLayout {
@@ -985,8 +1014,10 @@ hipError_t zero(void* out, size_t n, hipStream_t stream) {
   return hipErrorInvalidValue
 
 size_t embed_backward_workspace_bytes(int ntokens, int nrows, int channels) {
-  if (nrows <= kFewRows) return few_rows_bytes(ntokens, nrows, channels);
-  return sorted_layout(ntokens, nrows, channels).bytes;
+  // (whichever way is taken: that depends on the type and alignment of the call's arrays)
+  const size_t few = nrows <= kFewRows ? few_rows_bytes(ntokens, nrows, channels) : 0;
+  const size_t sorted = sorted_layout(ntokens, nrows, channels).bytes;
+  return few > sorted ? few : sorted;
 }
 
 hipError_t launch_embed(const TokenArg& t, const void* table, float scale, const float* scales,
@@ -1004,7 +1035,7 @@ hipError_t embed_backward(const TokenArg& t, const void* grad, const void* table
   bool scales_done = false;
   if (grad_table && t.nrows > 0 && t.channels > 0)
     e = t.ntokens == 0 ? zero<T>(grad_table, (size_t)t.nrows * t.channels, stream)
-        : t.nrows <= kFewRows
+        : copies_pay<T>(t, grad)
             ? few_rows<T, T, false>(t, grad, a, table, grad_scales, &scales_done, grad_table, (float*)workspace, nullptr,
                                     stream)
             : sorted_rows<T, T, false, false>(t, grad, a, grad_table, workspace, TableNorm(), stream);
@@ -1025,31 +1056,30 @@ hipError_t launch_embed_backward(const TokenArg& t, const void* grad, const void
 // encode's backward pass: rows in teams are summed and normed back in one launch; otherwise the sums
 // of all rows go through memory (first in the workspace), and layer_norm.hip takes them back.
 namespace {
-bool sums_in_memory(const TokenArg& t) {
-  return t.ntokens == 0 || t.nrows <= kFewRows || t.channels > kMostTeamChannels;
-}
 struct EncodeLayout {
   size_t params, named, rest, bytes;   // offsets: partial sums of weight and bias, bits of the rows that
                                        // tokens name, workspace of the row sums
 };
-EncodeLayout encode_layout(const TokenArg& t) {
+EncodeLayout encode_layout(int ntokens, int nrows, int channels, bool in_memory) {
   EncodeLayout l;
-  l.params = sums_in_memory(t) ? round_up((size_t)t.nrows * t.channels * sizeof(float)) : 0;
-  l.named = l.params + round_up(sums_in_memory(t)
-                                    ? norm_backward_workspace_bytes(t.nrows, t.channels)
-                                    : (size_t)(t.nrows < kRowParts ? t.nrows : kRowParts) * 2 * t.channels * sizeof(float));
-  l.rest = l.named + (t.nrows <= kFewRows ? kFewRowsParts * sizeof(uint32_t) : 0);
-  l.bytes = l.rest + (t.ntokens ? embed_backward_workspace_bytes(t.ntokens, t.nrows, t.channels) : 0);
+  l.params = in_memory ? round_up((size_t)nrows * channels * sizeof(float)) : 0;
+  l.named = l.params + round_up(in_memory
+                                    ? norm_backward_workspace_bytes(nrows, channels)
+                                    : (size_t)(nrows < kRowParts ? nrows : kRowParts) * 2 * channels * sizeof(float));
+  l.rest = l.named + (nrows <= kFewRows ? kFewRowsParts * sizeof(uint32_t) : 0);
+  l.bytes = l.rest + (ntokens ? embed_backward_workspace_bytes(ntokens, nrows, channels) : 0);
   return l;
 }
 template <typename T>
 hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad, const void* table, float scale,
                            const DropArg& drop, void* grad_table, void* grad_weight, void* grad_bias,
                            char* workspace, hipStream_t stream) {
-  const EncodeLayout l = encode_layout(t);
+  const bool copies = t.ntokens > 0 && t.nrows > 0 && copies_pay<T>(t, grad);
+  const bool in_memory = t.ntokens == 0 || t.nrows == 0 || copies || t.channels > kMostTeamChannels;
+  const EncodeLayout l = encode_layout(t.ntokens, t.nrows, t.channels, in_memory);
   const SumArg a{1.f, nullptr, drop};
   float* params = reinterpret_cast<float*>(workspace + l.params);
-  if (!sums_in_memory(t)) {
+  if (!in_memory) {
     const TableNorm norm{table, scale, n, grad_table != nullptr, grad_weight || grad_bias,
                          {params, grad_weight, grad_bias, n.param_dtype == MG_FLOAT32}};
     return sorted_rows<T, T, true, true>(t, grad, a, grad_table, workspace + l.rest, norm, stream);
@@ -1057,10 +1087,10 @@ hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad
   float* sums = reinterpret_cast<float*>(workspace);
   // which rows tokens name: the others have no part in the gradients, whatever stands in them
   NamedRows named{reinterpret_cast<uint32_t*>(workspace + l.named), 0, nullptr};
-  if (t.nrows > kFewRows && t.ntokens > 0) named = NamedRows{nullptr, 0, reinterpret_cast<int32_t*>(workspace + l.rest)};
+  if (!copies && t.ntokens > 0 && t.nrows > 0) named = NamedRows{nullptr, 0, reinterpret_cast<int32_t*>(workspace + l.rest)};
   hipError_t e = t.nrows == 0 ? hipSuccess
                  : t.ntokens == 0 ? zero<float>(sums, (size_t)t.nrows * t.channels, stream)
-                 : t.nrows <= kFewRows
+                 : copies
                      ? few_rows<T, float, true>(t, grad, a, nullptr, nullptr, nullptr, sums, (float*)(workspace + l.rest),
                                                 &named, stream)
                      : sorted_rows<T, float, true, false>(t, grad, a, sums, workspace + l.rest, TableNorm(), stream);
@@ -1070,11 +1100,11 @@ hipError_t encode_backward(const TokenArg& t, const NormArg& n, const void* grad
 }  // namespace
 
 size_t encode_backward_workspace_bytes(int ntokens, int nrows, int channels) {
-  TokenArg t{};
-  t.ntokens = ntokens;
-  t.nrows = nrows;
-  t.channels = channels;
-  return encode_layout(t).bytes;
+  const bool wide = channels > kMostTeamChannels;   // (whichever ways a call of these sizes can take)
+  const size_t in_memory =
+      ntokens == 0 || nrows <= kFewRows || wide ? encode_layout(ntokens, nrows, channels, true).bytes : 0;
+  const size_t other = ntokens == 0 || wide ? 0 : encode_layout(ntokens, nrows, channels, false).bytes;
+  return in_memory > other ? in_memory : other;
 }
 hipError_t launch_encode_backward(const TokenArg& t, const NormArg& a, const void* grad, const void* table,
                                   float scale, const DropArg& drop, void* grad_table, void* grad_weight,

@@ -22,7 +22,7 @@ constexpr int kMostTeamChannels = 8192;   // of rows that a team can hold
 // Calls f with the shape for rows of `packs` packs.  Few elements a lane (up to 32 of 16-bit types, 16
 // of any other) leave room for many waves, whose loads hide one another; four-wave teams pay with a
 // barrier a sum.  1001 channels of float16, one element a pack: 64 lanes of 16 packs take 16 us where
-// 256 lanes of four take 8 (4099 rows).  False: no team is wide enough.
+// 256 lanes of four take 10 (4099 rows).  False: no team is wide enough.
 template <int VEC, typename F>
 bool with_team(int packs, F f) {
   if constexpr (VEC == 1) {

@@ -54,6 +54,7 @@ EMBED = [
     ((40,), 9, 2056, BF16, torch.int32, True), ((9,), 4, 4099, F32, torch.int64, False),
     ((700,), 3, 16, F32, F32, True), ((700,), 513, 5, F16, torch.int32, False),
     ((2500,), 40, 12, BF16, torch.int64, True), ((2100,), 3000, 24, F32, torch.int64, False),
+    ((500,), 28, 300, F32, torch.int64, True), ((400,), 20, 1024, BF16, F32, False), ((3000,), 32, 24, F32, F32, True),
 ]
 
 
@@ -299,6 +300,8 @@ ENCODE = [
     ((12,), 30, 2048, BF16, F32, torch.int64, 0.1), ((5,), 3, 9001, F32, F32, torch.int32, 0.2),
     ((0,), 4, 8, F32, F32, F32, 0.1), ((5,), 0, 8, F32, F32, F32, 0.1), ((4000,), 28, 8, F32, F32, F32, 0.1),
     ((3000,), 700, 24, BF16, F32, torch.int64, 0.1), ((9,), 2, 1, F32, F32, F32, 1.0),
+    ((500,), 28, 300, F32, F32, torch.int64, 0.3), ((400,), 20, 1024, BF16, F32, F32, 0.1),
+    ((60,), 20, 8200, F16, F32, torch.int32, 0.1),
 ]
 
 
