@@ -12,6 +12,9 @@ SOURCES = ["capi.hip", "transform.hip", "convert.hip", "forward_sorted.hip", "fo
            "forward_vector_mfma.hip", "backward.hip", "second_order.hip", "interpolate.hip",
            "embed.hip", "layer_norm.hip", "dropout.hip"]
 
+# sources of very many kernel instances: minutes of compile time each when optimised, seconds without
+UNOPTIMISED = ("embed.hip", "layer_norm.hip")
+
 # EMU_SANITIZE selects a second build of the same sources with clang's run-time checks, every report
 # fatal: "1" the undefined-behaviour checks (array indices of fixed-size arrays -- the register and
 # LDS arrays of the kernels --, shifts, signed overflow, float-to-int conversions out of range,
@@ -72,6 +75,8 @@ def build(force=False, verbose=False):
     for src in SOURCES:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         cmd = [cxx, "-x", "c++"] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
+        if src in UNOPTIMISED:
+            cmd.append("-O0")
         procs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
                                                  stderr=subprocess.STDOUT, text=True)))
     rt = os.path.join(objdir, "hip_emu.o")

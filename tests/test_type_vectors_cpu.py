@@ -186,22 +186,24 @@ def test_host_layer_needs_a_device_or_says_so():
 # the kernels on the emulated device
 # ------------------------------------------------------------------------------------------------
 def test_drawn_cases(emulated_library):
-    p = emulated(["type_vectors.py", "60", "7"])
-    assert p.returncode == 0 and "60 rounds passed" in p.stdout, p.stdout[-3000:]
+    p = emulated(["type_vectors.py", "25", "7"])
+    assert p.returncode == 0 and "25 rounds passed" in p.stdout, p.stdout[-3000:]
 
 
-@pytest.mark.parametrize("env", [{"EMU_ORDER": "reverse"}, {"EMU_APPROX": "hash"}, {"EMU_CONTRACT": "1"}])
+@pytest.mark.parametrize("env", [{"EMU_ORDER": "reverse"}, {"EMU_APPROX": "hash"}, {"EMU_CONTRACT": "1"},
+                                 {"EMU_SANITIZE": "1"},
+                                 {"EMU_SANITIZE": "address", "ASAN_OPTIONS": "verify_asan_link_order=0:detect_leaks=0"}])
 def test_drawn_cases_in_other_modes(emulated_library, env):
     """Threads and workgroups last to first; approximate instructions one unit off; fused
-    multiply-adds."""
-    p = emulated(["type_vectors.py", "20", "8"], env)
-    assert p.returncode == 0 and "20 rounds passed" in p.stdout, p.stdout[-3000:]
+    multiply-adds; clang's run-time checks of undefined behaviour and of addresses."""
+    p = emulated(["type_vectors.py", "8", "8"], env)
+    assert p.returncode == 0 and "8 rounds passed" in p.stdout, p.stdout[-3000:]
 
 
 def test_device_tests_on_the_emulated_device(emulated_library):
-    """The GPU test file's cases of the functions (what needs autograd on device tensors, streams or
-    graphs is left to the device)."""
+    """Some of the GPU test file's cases of the functions (what needs autograd on device tensors, streams or
+    graphs is left to the device; all of the others pass here as well, in five minutes)."""
     p = emulated(["gpu_tests_on_fake_device.py", os.path.join(HERE, "test_type_vectors_gpu.py"), "-m", "gpu", "-q",
-                  "-x", "-k", "(embedding or unusual or name_no_row or dropout or encoding or layer_norm) and not "
-                  "many_rows and not module and not state"])
+                  "-x", "-k", "(unusual or name_no_row or no_part or hides or off_alignment or large_mean or "
+                  "without_spread or of_nothing or parts_one_after) and not 9001"])
     assert p.returncode == 0 and "passed" in p.stdout, p.stdout[-3000:]
