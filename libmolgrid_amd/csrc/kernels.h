@@ -6,7 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include "device_common.h"
-#include "element_types.h"
+#include "type_vector_args.h"
 
 namespace mg {
 
