@@ -418,20 +418,38 @@ def _new_seed():
 
 
 class _Drawing(torch.nn.Module):
-    """Seed and offset of a module that drops: every call while training takes the next offset.
-    ``state``, an int64 tensor (seed, offset) on the device, replaces them for calls that are
-    captured into a graph; whoever replays the graph changes it between the replays (or inside it,
-    behind the backward pass)."""
+    """Seed and offsets of a module that drops.
+
+    With a seed, call k while training has offset k.  Without one the seed comes from the package's
+    random source and every call draws its offset from torch's generator of the host, which
+    activation checkpointing restores before it runs a call again (unless told not to,
+    ``preserve_rng_state``): the repeated call drops the same elements.  A count cannot know of the
+    repetition, so a module with a seed refuses calls during a backward pass; a call that is given
+    its ``offset`` takes that one in any case.
+
+    ``state``, an int64 tensor (seed, offset) on the device, replaces seed and offset for calls that
+    are captured into a graph; whoever replays the graph changes it between the replays (or inside
+    it, behind the backward pass)."""
 
     def _open(self, p, seed, state):
         if not 0 <= float(p) <= 1:
             raise ValueError("p: expected a probability, got %r" % p)
         self.p = float(p)
+        self._counts = seed is not None
         self.seed = _new_seed() if seed is None else int(seed)
-        self.offset = 0
+        self.offset = 0      # calls so far, where they are counted
         self.state = state
 
-    def _numbers(self, on_device):
+    def _next_offset(self):
+        if not self._counts:
+            return int(torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("a call during a backward pass, which may repeat an earlier one: give "
+                               "the call its offset, or the module no seed")
+        self.offset += 1
+        return self.offset - 1
+
+    def _numbers(self, on_device, offset):
         """(p, seed, offset, state) of the next call"""
         if not self.training or self.p == 0:
             return 0.0, 0, 0, None
@@ -440,8 +458,7 @@ class _Drawing(torch.nn.Module):
         if on_device and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured graph would drop the same elements in every replay: "
                                "give the module a state tensor")
-        self.offset += 1
-        return self.p, self.seed, self.offset - 1, None
+        return self.p, self.seed, self._next_offset() if offset is None else int(offset), None
 
 
 class TypeEmbedding(torch.nn.Module):
@@ -482,14 +499,14 @@ class TypeNorm(torch.nn.Module):
 
 class TypeDropout(_Drawing):
     """Drops elements of type vectors while training (see ``dropout``); every call takes other
-    random numbers.  Without a seed one is drawn from the package's random source."""
+    random numbers: a count with a seed, torch's generator without one."""
 
     def __init__(self, p=0.1, seed=None, state=None):
         super().__init__()
         self._open(p, seed, state)
 
-    def forward(self, x):
-        p, seed, offset, state = self._numbers(x.is_cuda)
+    def forward(self, x, offset=None):
+        p, seed, offset, state = self._numbers(x.is_cuda, offset)
         return x if p == 0 else TypeDropoutFunction.apply(x.contiguous(), p, seed, offset, state)
 
     def extra_repr(self):
@@ -512,8 +529,8 @@ class TypeEncoder(_Drawing):
         self.scale, self.eps = float(scale), _eps(eps)
         torch.nn.init.normal_(self.weight)
 
-    def forward(self, type_index):
-        p, seed, offset, state = self._numbers(self.weight.is_cuda)
+    def forward(self, type_index, offset=None):
+        p, seed, offset, state = self._numbers(self.weight.is_cuda, offset)
         return TypeEncoderFunction.apply(type_index.contiguous(), self.weight.contiguous(),
                                          self.norm_weight, self.norm_bias, self.scale, self.eps, p,
                                          seed, offset, state)
