@@ -22,6 +22,7 @@ Everything runs on torch's current stream, nothing synchronises.
 """
 import functools
 import math
+import threading
 
 import numpy as np
 import torch
@@ -417,6 +418,23 @@ def _new_seed():
     return int(_gr._rng.integers(0, 2 ** 63))
 
 
+class _Calls(object):
+    """Number of a module's calls so far.  Replicas of the module (nn.DataParallel makes new ones for every
+    step) go on with the same one, copies with one of their own."""
+
+    def __init__(self, made=0):
+        self.made = made
+        self.lock = threading.Lock()
+
+    def __reduce__(self):
+        return _Calls, (self.made,)
+
+    def take(self):
+        with self.lock:
+            self.made += 1
+            return self.made - 1
+
+
 class _Drawing(torch.nn.Module):
     """Seed and offsets of a module that drops.
 
@@ -437,8 +455,17 @@ class _Drawing(torch.nn.Module):
         self.p = float(p)
         self._counts = seed is not None
         self.seed = _new_seed() if seed is None else int(seed)
-        self.offset = 0      # calls so far, where they are counted
+        self._calls = _Calls()
         self.state = state
+
+    @property
+    def offset(self):
+        """Calls so far of a module with a seed: the offset of the next one"""
+        return self._calls.made
+
+    @offset.setter
+    def offset(self, value):
+        self._calls.made = int(value)
 
     def _next_offset(self):
         if not self._counts:
@@ -446,8 +473,7 @@ class _Drawing(torch.nn.Module):
         if torch._C._current_graph_task_id() != -1:
             raise RuntimeError("a call during a backward pass, which may repeat an earlier one: give "
                                "the call its offset, or the module no seed")
-        self.offset += 1
-        return self.offset - 1
+        return self._calls.take()
 
     def _numbers(self, on_device, offset):
         """(p, seed, offset, state) of the next call"""

@@ -1,5 +1,7 @@
 """The random numbers that the type vectors' modules take, call by call: which calls have to agree
 (a call that activation checkpointing runs again) and which have to differ.  The host layer alone: the mask comes from the plain form, so no device is needed."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -127,3 +129,24 @@ def test_calls_differ_and_a_seed_counts(mg):
     drop(x), drop(x, offset=5), mg.TypeDropout(0.0)(x), mg.TypeDropout(0.5).eval()(x)
     assert torch.equal(before, torch.get_rng_state())           # nothing drawn that is not needed
     assert drop.offset == 4
+
+
+@pytest.mark.parametrize("seed", [None, 6])
+def test_replicas_move_the_module_on(mg, seed):
+    """Replicas are made anew for every step (as DataParallel makes them): their calls count."""
+    x, _ = _inputs(4096)
+    drop = mg.TypeDropout(0.5, seed=seed)
+    steps = [drop._replicate_for_data_parallel()(x) for _ in range(3)]
+    for i in range(3):
+        for j in range(i):
+            assert not torch.equal(steps[i], steps[j])
+
+
+def test_copies_count_for_themselves(mg):
+    x, _ = _inputs(4096)
+    drop = mg.TypeDropout(0.5, seed=6)
+    drop(x)
+    copied = copy.deepcopy(drop)
+    assert torch.equal(copied(x), drop(x))
+    copied(x)
+    assert (copied.offset, drop.offset) == (3, 2)
