@@ -443,7 +443,7 @@ class _Drawing(torch.nn.Module):
     activation checkpointing restores before it runs a call again (unless told not to,
     ``preserve_rng_state``): the repeated call drops the same elements.  A count cannot know of the
     repetition, so a module with a seed refuses calls during a backward pass; a call that is given
-    its ``offset`` takes that one in any case.
+    its ``offset`` takes that one in any case.  Seed and count are part of the module's state_dict.
 
     ``state``, an int64 tensor (seed, offset) on the device, replaces seed and offset for calls that
     are captured into a graph; whoever replays the graph changes it between the replays (or inside
@@ -455,6 +455,8 @@ class _Drawing(torch.nn.Module):
         self.p = float(p)
         self._counts = seed is not None
         self.seed = _new_seed() if seed is None else int(seed)
+        if not 0 <= self.seed < 2 ** 64:
+            raise ValueError("seed: expected a number of 64 bits")
         self._calls = _Calls()
         self.state = state
 
@@ -485,6 +487,21 @@ class _Drawing(torch.nn.Module):
             raise RuntimeError("a captured graph would drop the same elements in every replay: "
                                "give the module a state tensor")
         return self.p, self.seed, self._next_offset() if offset is None else int(offset), None
+
+    def get_extra_state(self):
+        """(seed, calls so far), 64 bits each"""
+        seed = self.seed - 2 ** 64 if self.seed >= 2 ** 63 else self.seed
+        return torch.tensor([seed, self._calls.made], dtype=torch.int64, device="cpu")
+
+    def set_extra_state(self, state):
+        seed, made = (int(n) for n in state)
+        self.seed, self._calls.made = seed % 2 ** 64, made
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, *others):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, *others)
+        key = prefix + "_extra_state"
+        if key in missing_keys:     # (of a module that kept no numbers: those here stay)
+            missing_keys.remove(key)
 
 
 class TypeEmbedding(torch.nn.Module):

@@ -1,6 +1,8 @@
 """The random numbers that the type vectors' modules take, call by call: which calls have to agree
-(a call that activation checkpointing runs again) and which have to differ.  The host layer alone: the mask comes from the plain form, so no device is needed."""
+(a call that activation checkpointing runs again, a module saved and loaded) and which have to
+differ.  The host layer alone: the mask comes from the plain form, so no device is needed."""
 import copy
+import io
 
 import numpy as np
 import pytest
@@ -150,3 +152,31 @@ def test_copies_count_for_themselves(mg):
     assert torch.equal(copied(x), drop(x))
     copied(x)
     assert (copied.offset, drop.offset) == (3, 2)
+
+
+@pytest.mark.parametrize("seed", [0, 5, 2 ** 63, 2 ** 64 - 1])
+def test_a_loaded_module_goes_on_where_the_saved_one_was(mg, seed):
+    x, _ = _inputs(4096)
+    drop = mg.TypeDropout(0.5, seed=seed)
+    drop(x), drop(x)
+    file = io.BytesIO()
+    torch.save(torch.nn.Sequential(drop).state_dict(), file)
+    file.seek(0)
+    resumed = mg.TypeDropout(0.5, seed=1)
+    torch.nn.Sequential(resumed).load_state_dict(torch.load(file, weights_only=True))
+    assert (resumed.seed, resumed.offset) == (seed, 2)
+    assert torch.equal(resumed(x), drop(x))
+    for bad in (-1, 2 ** 64):
+        with pytest.raises(ValueError):
+            mg.TypeDropout(0.5, seed=bad)
+
+
+def test_a_state_dict_without_numbers_is_loaded(mg):
+    encoder = mg.TypeEncoder(5, 8, p=0.5, seed=3)
+    saved = {k: v for k, v in encoder.state_dict().items() if not k.endswith("_extra_state")}
+    assert len(saved) == 3
+    other = mg.TypeEncoder(5, 8, p=0.5, seed=4)
+    other.load_state_dict(saved)
+    assert other.seed == 4 and torch.equal(other.weight, encoder.weight)
+    with pytest.raises(RuntimeError):
+        other.load_state_dict({k: v for k, v in saved.items() if k != "norm_bias"})
