@@ -387,8 +387,9 @@ int mg_layer_norm_backward(int nrows, int channels, int dtype, int param_dtype, 
  * are at least T: half e % 8 (the low half of a word first) of the four words that
  * Philox4x32 with ten rounds gives for the counter (e / 8, offset) and the key
  * seed.  The mask is stored nowhere: the backward pass is the same call on the
- * gradient.  `state` (device, two uint64: seed, offset) replaces the two numbers
- * when it is not NULL, for graphs that are replayed with other numbers.
+ * gradient.  `state` (device, two uint64), when it is not NULL, is added to seed and
+ * offset, modulo 2^64, for graphs that are replayed with other numbers: calls that
+ * share a state keep masks of their own by their seeds or offsets.
  * out == in is allowed. */
 int mg_dropout(uint64_t n, int dtype, const void* in, double p, uint64_t seed, uint64_t offset,
                const uint64_t* state, void* out, void* stream);

@@ -149,8 +149,8 @@ __device__ __forceinline__ Words4 philox(uint64_t low, uint64_t high, uint64_t k
 }
 
 __device__ __forceinline__ void drop_key(const DropArg& a, uint64_t& seed, uint64_t& offset) {
-  seed = a.state ? a.state[0] : a.seed;
-  offset = a.state ? a.state[1] : a.offset;
+  seed = a.seed + (a.state ? a.state[0] : 0);   // (modulo 2^64)
+  offset = a.offset + (a.state ? a.state[1] : 0);
 }
 __device__ __forceinline__ uint32_t drop_half(const Words4& words, int i) {
   return i & 1 ? words.w[i >> 1] >> 16 : words.w[i >> 1] & 0xFFFFu;

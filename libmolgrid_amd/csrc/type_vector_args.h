@@ -31,8 +31,8 @@ struct NormArg {
 struct DropArg {
   uint32_t limit;         // round(65536 p): 0 keeps everything, 65536 nothing
   float factor;           // 65536 / (65536 - limit), 0 when nothing is kept
-  uint64_t seed, offset;  // unless state is given
-  const uint64_t* state;  // device: {seed, offset}
+  uint64_t seed, offset;
+  const uint64_t* state;  // device: two numbers that are added to them, or nullptr
 };
 
 // Which rows of a table tokens name: by bits (of up to 32 rows, in `count` words that are ORed

@@ -279,8 +279,8 @@ def dropout(x, p, seed=0, offset=0, state=None):
     that the expectation stays; p counts in steps of 2^-16.  Which elements are kept is a function
     of (seed, offset) and their position in the flattened tensor: other calls take another seed or
     offset (numbers of 64 bits), the backward pass the same ones on the gradient.  ``state``, an
-    int64 tensor (seed, offset) on the device, replaces the two, so that a captured graph can be
-    replayed with other numbers."""
+    int64 tensor of two numbers on the device, is added to seed and offset (modulo 2^64), so that a
+    captured graph can be replayed with other numbers."""
     x = _tensor(x, "x", _DTYPES)
     p, seed, offset, state_ptr = _drop_args(p, seed, offset, state)
     out = torch.empty_like(x)
@@ -445,9 +445,11 @@ class _Drawing(torch.nn.Module):
     repetition, so a module with a seed refuses calls during a backward pass; a call that is given
     its ``offset`` takes that one in any case.  Seed and count are part of the module's state_dict.
 
-    ``state``, an int64 tensor (seed, offset) on the device, replaces seed and offset for calls that
-    are captured into a graph; whoever replays the graph changes it between the replays (or inside
-    it, behind the backward pass)."""
+    ``state``, an int64 tensor of two numbers on the device, is added to the seed and to an offset of 0
+    (or the one that the call is given), for calls that are captured into a graph; whoever replays the
+    graph changes it between the replays (or inside it, behind the backward pass).  Modules that share
+    a state drop other elements by their seeds; several calls of one module under the same numbers are
+    given an offset each."""
 
     def _open(self, p, seed, state):
         if not 0 <= float(p) <= 1:
@@ -482,7 +484,7 @@ class _Drawing(torch.nn.Module):
         if not self.training or self.p == 0:
             return 0.0, 0, 0, None
         if self.state is not None:
-            return self.p, 0, 0, self.state
+            return self.p, self.seed, 0 if offset is None else int(offset), self.state
         if on_device and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured graph would drop the same elements in every replay: "
                                "give the module a state tensor")

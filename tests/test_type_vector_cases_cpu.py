@@ -1,0 +1,15 @@
+"""Fixed cases of the type vectors' kernels on the emulated device (tests/emu/type_vector_cases.py)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+RUNNER = os.path.join(os.path.dirname(os.path.abspath(__file__)), "emu", "type_vector_cases.py")
+
+
+@pytest.mark.parametrize("name", ["numbers_beside_a_state"])
+def test_case(name):
+    p = subprocess.run([sys.executable, RUNNER, name], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                       text=True, timeout=600)
+    assert p.returncode == 0 and name + " passed" in p.stdout, p.stdout[-3000:]

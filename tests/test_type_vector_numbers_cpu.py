@@ -19,7 +19,7 @@ def mg(monkeypatch):
 
     def dropout(x, p, seed=0, offset=0, state=None):
         if state is not None:
-            seed, offset = (int(n) % 2 ** 64 for n in state)
+            seed, offset = ((int(n) + m) % 2 ** 64 for n, m in zip(state, (seed, offset)))
         keep, factor = ref.kept(x.numel(), p, seed, offset)
         mask = torch.from_numpy(keep.reshape(tuple(x.shape)))
         return torch.where(mask, x * factor, torch.zeros((), dtype=x.dtype))
@@ -180,3 +180,19 @@ def test_a_state_dict_without_numbers_is_loaded(mg):
     assert other.seed == 4 and torch.equal(other.weight, encoder.weight)
     with pytest.raises(RuntimeError):
         other.load_state_dict({k: v for k, v in saved.items() if k != "norm_bias"})
+
+
+def test_modules_that_share_a_state_drop_other_elements(mg):
+    """A state is added to the module's own numbers, whether the seed was given or drawn, and to the offset
+    that a call is given."""
+    x, _ = _inputs(4096)
+    state = torch.tensor([100, -1])
+    drops = [mg.TypeDropout(0.5, seed=3, state=state), mg.TypeDropout(0.5, seed=4, state=state),
+             mg.TypeDropout(0.5, state=state), mg.TypeDropout(0.5, state=state)]
+    masks = [drop(x).detach() != 0 for drop in drops] + [drops[0](x, offset=1).detach() != 0]
+    for i, mask in enumerate(masks):
+        assert all(not torch.equal(mask, other) for other in masks[:i])
+    assert np.array_equal(masks[0].numpy(), ref.kept(4096, 0.5, 103, 2 ** 64 - 1)[0])
+    assert np.array_equal(masks[4].numpy(), ref.kept(4096, 0.5, 103, 0)[0])
+    for drop, mask in zip(drops, masks):                        # the same numbers: the same elements
+        assert torch.equal(drop(x).detach() != 0, mask)

@@ -55,3 +55,26 @@ def test_a_counted_call_says_which_it_is(mg, reentrant):
     checkpoint(lambda t: drop(t, offset=7) * w, x, use_reentrant=reentrant).sum().backward()
     keep = torch.from_numpy(ref.kept(3001, 0.5, 4, 7)[0] * 2.0).float().cuda()
     assert torch.equal(w.grad, keep * x.detach()) and torch.equal(x.grad, keep * w.detach())
+
+
+def test_modules_that_share_a_state_in_one_graph(mg):
+    """Two modules and a second call of one of them, captured together: masks of their own in every replay, those
+    of the plain form for seed and offset with the state added."""
+    x = torch.ones(4099).cuda()
+    state = torch.tensor([0, 0]).cuda()
+    first, second = mg.TypeDropout(0.5, seed=2 ** 64 - 5, state=state), mg.TypeDropout(0.25, seed=2, state=state)
+    calls = ((first, None, 2 ** 64 - 5, 0.5), (second, None, 2, 0.25), (first, 6, 2 ** 64 - 5, 0.5))
+    for module, offset, _, _ in calls:      # (loads the kernels before the capture)
+        module(x, offset=offset)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = [module(x, offset=offset) for module, offset, _, _ in calls]
+    for replay in range(4):
+        state.copy_(torch.tensor([100 * replay + 11, -replay]).cuda())
+        graph.replay()
+        torch.cuda.synchronize()
+        for out, (module, offset, seed, p) in zip(outputs, calls):
+            keep, factor = ref.kept(4099, p, (seed + 100 * replay + 11) % 2 ** 64, ((offset or 0) - replay) % 2 ** 64)
+            assert torch.equal(out.cpu(), torch.from_numpy(keep * factor).float()), replay
+            assert torch.equal(out, module(x, offset=offset)), replay
