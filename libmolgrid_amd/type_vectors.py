@@ -125,6 +125,7 @@ def _table_args(type_index, table):
 
 def _scale_args(scale, index):
     """(number, per-token tensor or None)"""
+    scale = _gr._unwrap(scale)
     if _is_array(scale):
         scale = _tensor(scale, "scale", (torch.float32,))
         if scale.shape != index.shape:
@@ -137,7 +138,7 @@ def _scale_args(scale, index):
 def _param(x, name, channels, dtype, like=None):
     if x is None:
         return None
-    _tensor(x, name, _DTYPES)
+    x = _tensor(x, name, _DTYPES)
     if x.shape != (channels,):
         raise ValueError("%s: expected shape (%d,), got %s" % (name, channels, tuple(x.shape)))
     if x.dtype not in (torch.float32, dtype) or (like is not None and x.dtype != like.dtype):
@@ -151,14 +152,14 @@ def _param_gradients(weight, channels, like):
 
 
 def _like(grad, name, shape, dtype):
-    _tensor(grad, name, (dtype,))
+    grad = _tensor(grad, name, (dtype,))
     if grad.shape != shape:
         raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(grad.shape)))
     return grad
 
 
 def _number(x, name):
-    if _is_array(x):
+    if _is_array(_gr._unwrap(x)):
         raise ValueError("%s: expected a number" % name)
     return float(x)
 
@@ -175,7 +176,7 @@ def _drop_args(p, seed, offset, state):
     if not 0 <= p <= 1:
         raise ValueError("p: expected a probability, got %r" % p)
     if state is not None:
-        _tensor(state, "state", (torch.int64,))
+        state = _tensor(state, "state", (torch.int64,))
         if tuple(state.shape) != (2,):
             raise ValueError("state: expected two numbers, seed and offset")
     seed, offset = int(seed), int(offset)

@@ -13,3 +13,11 @@ def test_case(name):
     p = subprocess.run([sys.executable, RUNNER, name], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                        text=True, timeout=600)
     assert p.returncode == 0 and name + " passed" in p.stdout, p.stdout[-3000:]
+
+
+def test_views_on_the_emulated_device():
+    here = os.path.dirname(RUNNER)
+    p = subprocess.run([sys.executable, os.path.join(here, "gpu_tests_on_fake_device.py"),
+                        os.path.join(os.path.dirname(here), "test_type_vector_views_gpu.py"), "-m", "gpu", "-q"],
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=600)
+    assert p.returncode == 0 and "2 passed" in p.stdout, p.stdout[-3000:]
