@@ -12,7 +12,8 @@ SOURCES = ["capi.hip", "transform.hip", "convert.hip", "forward_sorted.hip", "fo
            "forward_vector_mfma.hip", "backward.hip", "second_order.hip", "interpolate.hip",
            "embed.hip", "layer_norm.hip", "dropout.hip"]
 
-# sources of very many kernel instances: minutes of compile time each when optimised, seconds without
+# sources of very many kernel instances: a minute or two of compile time each when optimised, seconds without
+# (the contracting build has to optimise them: without, the compiler fuses nothing)
 UNOPTIMISED = ("embed.hip", "layer_norm.hip")
 
 # EMU_SANITIZE selects a second build of the same sources with clang's run-time checks, every report
@@ -76,7 +77,7 @@ def build(force=False, verbose=False):
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         cmd = [cxx, "-x", "c++"] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
         if src in UNOPTIMISED:
-            cmd.append("-O0")
+            cmd.append("-g0" if CONTRACT else "-O0")
         procs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
                                                  stderr=subprocess.STDOUT, text=True)))
     rt = os.path.join(objdir, "hip_emu.o")

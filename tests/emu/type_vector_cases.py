@@ -43,6 +43,26 @@ def numbers_beside_a_state():
         check(back(to_table, torch.float32), *dt, torch.float32, "gradient of the table")
 
 
+def digest():
+    """Prints digests of the gradients that both sources compute with products and sums: layer norm's of its input (whose
+    forward pass has no product that could be fused), and an encoder's of its table by sorted tokens."""
+    import hashlib
+    rng = np.random.default_rng(3)
+    rows, channels = 60, 96
+    a_x, a_grad = (put(values(rng, (rows, channels), torch.float32, 2.0, 0.7)) for _ in range(2))
+    a_weight, index = put(values(rng, channels, torch.float32)), put(torch.arange(rows))
+    a_mean, a_rstd = put(values(rng, rows, torch.float32)), put(values(rng, rows, torch.float32, 0.1, 1.0))
+    to_x, to_table = (place((rows, channels), torch.float32) for _ in range(2))
+    ok(e.lib.mg_layer_norm_backward(rows, channels, 0, 0, e.ptr(a_grad), e.ptr(a_x), e.ptr(a_mean), e.ptr(a_rstd),
+                                    e.ptr(a_weight), e.ptr(to_x), None, None, None, 0, None))
+    w, size = workspace(e.lib.mg_encode_types_backward_workspace_size(rows, rows, channels))
+    ok(e.lib.mg_encode_types_backward(rows, rows, channels, 0, 0, KINDS.index(torch.int64), e.ptr(index), e.ptr(a_grad),
+                                      e.ptr(a_x), 1.3, e.ptr(a_weight), 1e-5, 0.0, 0, 0, None, e.ptr(to_table), None,
+                                      None, w, size, None))
+    for what, a in (("layer_norm", to_x), ("embed", to_table)):
+        print(what, hashlib.sha256(np.ascontiguousarray(a).tobytes()).hexdigest())
+
+
 if __name__ == "__main__":
     for name in sys.argv[1:]:
         globals()[name]()

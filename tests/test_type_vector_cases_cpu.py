@@ -21,3 +21,15 @@ def test_views_on_the_emulated_device():
                         os.path.join(os.path.dirname(here), "test_type_vector_views_gpu.py"), "-m", "gpu", "-q"],
                        stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=600)
     assert p.returncode == 0 and "2 passed" in p.stdout, p.stdout[-3000:]
+
+
+def test_the_contracting_build_fuses_products_and_sums():
+    """EMU_CONTRACT=1 is for checks under fused multiply-adds: its results are not those of the build without."""
+    lines = []
+    for env in ({}, {"EMU_CONTRACT": "1"}):
+        p = subprocess.run([sys.executable, RUNNER, "digest"], env=dict(os.environ, **env), stdout=subprocess.PIPE,
+                           stderr=subprocess.STDOUT, text=True, timeout=1500)
+        assert p.returncode == 0, p.stdout[-3000:]
+        lines.append(p.stdout.splitlines())
+    for plain, contracted in zip(lines[0][:2], lines[1][:2]):
+        assert plain.split()[0] == contracted.split()[0] and plain != contracted
