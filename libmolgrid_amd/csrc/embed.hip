@@ -277,10 +277,10 @@ __global__ __launch_bounds__(kWave* kSumWaves) void sum_tables_kernel(
 //
 // Up to kOneLaunchTokens tokens are sorted by one launch (sort_tokens_kernel): a workgroup owns a range
 // of rows, reads every index and keeps those of its range.  Every compute unit reads all indices
-// then, and the workgroup of a frequent row has most of the placing to do: 7 us for 1,000 tokens,
-// 16 us for 16,384, 45 us for 65,536 and 181 us for 262,144 of a vocabulary (131,072 rows).  More
-// tokens are sorted by digits of their row, two launches for each of 9 bits, whose time hardly depends
-// on the tokens.  Both give the same order: rows ascending, and the tokens of a row as they were.
+// then, and the workgroup of a frequent row has most of the placing to do: 7 us for 1,000 tokens and
+// 16 us for 16,384 of a vocabulary (131,072 rows).  More tokens are sorted by digits of their row, two
+// or three launches for each of 9 bits.  Both give the same order: rows ascending, and the tokens of a
+// row as they were.
 // (Table gradients of eight floats a row, one launch and digits: 27 and 45 us for 12,000 tokens, 44 and
 // 51 us for 32,768.)
 constexpr int kOneLaunchTokens = 32768;
@@ -422,8 +422,13 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens_kernel(const I* __re
 // By digits: the tokens of a tile are counted by their digit, then every tile's workgroup works out
 // where each of its digits begins from all tiles' counts, ranks its tokens (those of a wave by the
 // lanes of equal digit, those of its waves one after the other) and moves them.  FIRST: the rows come
-// from the indices; a token without a row gets the row behind the last one.
+// from the indices; a token without a row gets the row behind the last one.  Every workgroup would read
+// the counts of every tile, which grows with the square of the tokens: beyond kMostTilesRead tiles a
+// launch between the two sums them over the tiles.  Table gradients of one float a row, 1,000 rows, counts
+// read and summed: 524,288 tokens (128 tiles) 64 and 67 us, 1,048,576 108 and 104, 4,194,304 515 and 370,
+// 16,777,216 3,810 and 1,350.
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kTile = 4096, kTileSteps = kTile / kSortThreads;
+constexpr int kMostTilesRead = 128;
 
 template <bool FIRST>
 __device__ __forceinline__ uint32_t tile_row(const TokenArg& t, const int32_t* rows, uint32_t i) {
@@ -447,7 +452,38 @@ __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(TokenArg t, 
   for (int i = threadIdx.x; i < kDigits; i += kSortThreads) counts[(size_t)blockIdx.x * kDigits + i] = count[i];
 }
 
-template <bool FIRST>
+// Counts [tiles][kDigits] become those of the tiles before, with the sum over all tiles behind the last: a
+// workgroup takes 64 digits, its waves a share of the tiles each.
+__global__ __launch_bounds__(kSortThreads) void sum_digits_kernel(int32_t* counts, int tiles) {
+  __shared__ int sums[kSortWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int share = (tiles + kSortWaves - 1) / kSortWaves;
+  const int begin = min(wave * share, tiles), end = min(begin + share, tiles);
+  int32_t* column = counts + blockIdx.x * kWave + lane;
+  int sum = 0;
+#pragma unroll 16
+  for (int k = begin; k < end; ++k) sum += column[(size_t)k * kDigits];
+  sums[wave][lane] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < wave; ++w) before += sums[w][lane];
+  constexpr int U = 16;   // loads in flight
+  for (int k0 = begin; k0 < end; k0 += U) {
+    int count[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) count[u] = column[(size_t)min(k0 + u, end - 1) * kDigits];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u >= end) break;
+      column[(size_t)(k0 + u) * kDigits] = before;
+      before += count[u];
+    }
+  }
+  if (wave == kSortWaves - 1) column[(size_t)tiles * kDigits] = before;
+}
+
+// SUMMED: the counts went through sum_digits_kernel.
+template <bool FIRST, bool SUMMED>
 __global__ __launch_bounds__(kSortThreads) void move_digits_kernel(
     TokenArg t, const int32_t* __restrict__ rows, const int32_t* __restrict__ order, int shift,
     const int32_t* __restrict__ counts, int32_t* __restrict__ to_rows, int32_t* __restrict__ to_order) {
@@ -458,11 +494,19 @@ __global__ __launch_bounds__(kSortThreads) void move_digits_kernel(
   // the tiles' counts of a digit: all of them, and those of the tiles before this one
   const int digit = threadIdx.x % kDigits, half = threadIdx.x / kDigits;
   int total = 0, before = 0;
+  if (SUMMED) {   // (a half of the workgroup one each, the halves are added)
+    const int v = counts[(size_t)(half ? gridDim.x : blockIdx.x) * kDigits + digit];
+    if (half)
+      total = v;
+    else
+      before = v;
+  } else {
 #pragma unroll 8
-  for (int k = half; k < (int)gridDim.x; k += kSortThreads / kDigits) {
-    const int v = counts[(size_t)k * kDigits + digit];
-    total += v;
-    before += k < (int)blockIdx.x ? v : 0;
+    for (int k = half; k < (int)gridDim.x; k += kSortThreads / kDigits) {
+      const int v = counts[(size_t)k * kDigits + digit];
+      total += v;
+      before += k < (int)blockIdx.x ? v : 0;
+    }
   }
   totals[half][digit] = total;
   befores[half][digit] = before;
@@ -863,7 +907,7 @@ SortedLayout sorted_layout(int ntokens, int nrows, int channels) {
   l.other_order = l.row + list;
   l.other_row = l.other_order + (l.tiles ? list : 0);
   l.counts = l.other_row + (l.tiles ? list : 0);
-  l.partial = l.counts + round_up((size_t)l.tiles * kDigits * sizeof(int32_t));
+  l.partial = l.counts + round_up(((size_t)l.tiles + (l.tiles > kMostTilesRead)) * kDigits * sizeof(int32_t));
   l.bytes = l.partial + round_up((size_t)l.slots * channels * sizeof(float));
   return l;
 }
@@ -914,17 +958,24 @@ Sorted sort_tokens(const TokenArg& t, const SortedLayout& l, char* base, hipStre
     for (int p = 0; p < passes; ++p) {
       const bool last = (passes - 1 - p) % 2 == 0;   // the last pass ends in `sorted`
       const Sorted &to = last ? sorted : other, &from = last ? other : sorted;
-      const dim3 grid(l.tiles), block(kSortThreads);
-      if (p == 0) {
-        hipLaunchKernelGGL(count_digits_kernel<true>, grid, block, 0, stream, t, nullptr, 0, list(l.counts));
-        hipLaunchKernelGGL(move_digits_kernel<true>, grid, block, 0, stream, t, nullptr, nullptr, 0,
-                           list(l.counts), to.row, to.order);
-      } else {
-        hipLaunchKernelGGL(count_digits_kernel<false>, grid, block, 0, stream, t, from.row, p * kDigitBits,
-                           list(l.counts));
-        hipLaunchKernelGGL(move_digits_kernel<false>, grid, block, 0, stream, t, from.row, from.order,
-                           p * kDigitBits, list(l.counts), to.row, to.order);
-      }
+      const auto pass = [&](auto first, const int32_t* rows, const int32_t* order) {
+        constexpr bool FIRST = decltype(first)::value;
+        const dim3 grid(l.tiles), block(kSortThreads);
+        int32_t* counts = list(l.counts);
+        hipLaunchKernelGGL(count_digits_kernel<FIRST>, grid, block, 0, stream, t, rows, p * kDigitBits, counts);
+        if (l.tiles > kMostTilesRead) {
+          hipLaunchKernelGGL(sum_digits_kernel, dim3(kDigits / kWave), block, 0, stream, counts, l.tiles);
+          hipLaunchKernelGGL((move_digits_kernel<FIRST, true>), grid, block, 0, stream, t, rows, order, p * kDigitBits,
+                             counts, to.row, to.order);
+        } else {
+          hipLaunchKernelGGL((move_digits_kernel<FIRST, false>), grid, block, 0, stream, t, rows, order, p * kDigitBits,
+                             counts, to.row, to.order);
+        }
+      };
+      if (p == 0)
+        pass(std::true_type(), nullptr, nullptr);
+      else
+        pass(std::false_type(), from.row, from.order);
     }
     hipLaunchKernelGGL(row_starts_kernel, dim3(((unsigned)t.ntokens + kThreads) / kThreads), dim3(kThreads), 0,
                        stream, t, sorted);

@@ -43,6 +43,24 @@ def numbers_beside_a_state():
         check(back(to_table, torch.float32), *dt, torch.float32, "gradient of the table")
 
 
+def many_tiles():
+    """Tokens of more tiles than the digit sort reads the counts of one by one, the last one ragged, two passes of
+    digits: whole numbers, so the sums are exact in any order."""
+    rng = np.random.default_rng(4)
+    tokens, rows = 129 * 4096 + 77, 600
+    at = rng.integers(-1, rows + 1, tokens)
+    at[:40000] = 3                                                # (a row that fills tiles)
+    grad = rng.integers(-8, 9, (tokens, 1)).astype(np.float32)
+    index, a_grad = put(torch.tensor(at, dtype=torch.int32)), e.put(grad)
+    to_table = place((rows, 1), torch.float32)
+    w, size = workspace(e.lib.mg_embed_types_backward_workspace_size(tokens, rows, 1))
+    ok(e.lib.mg_embed_types_backward(tokens, rows, 1, 0, KINDS.index(torch.int32), e.ptr(index), e.ptr(a_grad), None, 1.0,
+                                     None, e.ptr(to_table), None, w, size, None))
+    named = (at >= 0) & (at < rows)
+    expected = np.bincount(at[named], grad[named, 0].astype(np.float64), rows)
+    assert np.array_equal(to_table[:, 0], expected)
+
+
 def digest():
     """Prints digests of the gradients that both sources compute with products and sums: layer norm's of its input (whose
     forward pass has no product that could be fused), and an encoder's of its table by sorted tokens."""

@@ -8,7 +8,7 @@ import pytest
 RUNNER = os.path.join(os.path.dirname(os.path.abspath(__file__)), "emu", "type_vector_cases.py")
 
 
-@pytest.mark.parametrize("name", ["numbers_beside_a_state"])
+@pytest.mark.parametrize("name", ["numbers_beside_a_state", "many_tiles"])
 def test_case(name):
     p = subprocess.run([sys.executable, RUNNER, name], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                        text=True, timeout=600)
