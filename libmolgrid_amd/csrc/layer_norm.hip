@@ -87,7 +87,6 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
       const int row = live ? token_row(tokens, n) : -1;
       at = row < 0 ? 0 : row;
       live = next_named = row >= 0;
-      if (a.nrows == 0) return;
     }
     load_row<T, VEC, LANES, K>(x + at * channels, channels, lane, live, next);
   };
@@ -129,9 +128,26 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_kernel(
 
 // ENCODE with a table of few rows: every workgroup norms the table once, into LDS, and goes through
 // the result in groups of eight elements, each with one counter of the generator and one store,
-// whatever the channels are: 121,250 tokens, 28 rows of 32 floats in 9.4 us, a team a token takes 23 us.
+// whatever the channels are.
 constexpr int kFewRowsFloats = 8192;   // of a table: 32 KB
 constexpr size_t kFewRowsBlocks = 1024;
+constexpr int kFewRowsLanes = 8, kFewRowsTeams = kThreads / kFewRowsLanes;   // that share a row; rows normed at a time
+
+// Whether it pays.  Norming the table takes each workgroup about 0.5 us a round of kFewRowsTeams rows and 0.16 us
+// for every eight channels of one, which the tokens have to bring in: a team a token draws a counter for each pack,
+// so eight times as many where an element is a pack and twice as many for floats.  This kernel and a team
+// a token, us, 28 rows and 20,000 | 121,250 tokens unless said:
+//   one-element packs:   27 channels of bfloat16 6.5, 8.1 | 9.9, 33;  255 22, 18 | 45, 80;  300 rows of 27 22, 8.0 | 28, 34
+//   packs of floats:     32 channels 4.7, 4.4 | 8.9, 9.6;  256 16, 12 | 35, 44;  64 rows of 128 15, 7.6 | 26, 26
+//   packs of 16 bits:    32 channels 4.6, 4.3 | 7.2, 7.9;  256 15, 9.0 | 32, 29;  64 rows of 32 5.8, 4.3 | 9.0, 7.9
+// and few tokens of wide rows: 300 tokens, one row of 8,192 floats 202, 13.
+bool few_rows_pay(const TokenArg& t, size_t element, bool packs) {
+  if (t.nrows == 0) return true;   // zeros
+  if ((size_t)t.nrows * t.channels > (size_t)kFewRowsFloats) return false;
+  const int rounds = (t.nrows + kFewRowsTeams - 1) / kFewRowsTeams;
+  if (!packs) return t.ntokens >= 10000 * (rounds + 1);
+  return rounds == 1 && t.ntokens >= 50000 && (element == 4 || t.channels <= 64);
+}
 
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void few_rows_encode_kernel(
@@ -140,8 +156,7 @@ __global__ __launch_bounds__(kThreads) void few_rows_encode_kernel(
   HIP_DYNAMIC_SHARED(float, vectors);   // [nrows][channels]
   uint64_t seed, offset;
   drop_key(arg, seed, offset);
-  // eight lanes a row: a table of few rows goes through in one round
-  constexpr int LANES = 8, kTeams = kThreads / LANES;
+  constexpr int LANES = kFewRowsLanes, kTeams = kFewRowsTeams;
   const int lane = threadIdx.x % LANES, channels = t.channels;
   const bool is_float = a.param_dtype == MG_FLOAT32;
   for (int row0 = 0; row0 < t.nrows; row0 += kTeams) {
@@ -451,7 +466,8 @@ template <typename T, bool ENCODE>
 hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x, const void* bias,
                 const DropArg& drop, void* out, float* means, float* rstds, hipStream_t stream) {
   const uint32_t nrows = (uint32_t)(ENCODE ? t.ntokens : a.nrows);
-  if (ENCODE && t.nrows <= t.ntokens && (size_t)t.nrows * t.channels <= kFewRowsFloats) {
+  const bool packs = whole_packs<T>(a.channels, address(x) | address(out));
+  if (ENCODE && few_rows_pay(t, sizeof(T), packs)) {
     const size_t groups = ((size_t)t.ntokens * t.channels + 7) / 8;
     const size_t all = (groups + kThreads - 1) / kThreads, blocks = all < kFewRowsBlocks ? all : kFewRowsBlocks;
     const size_t step = blocks * kThreads * 8, shared = (size_t)t.nrows * t.channels * sizeof(float);
@@ -477,9 +493,8 @@ hipError_t norm(const NormArg& a, const TokenArg& t, float scale, const void* x,
                          (const T*)x, t, scale, a, bias, drop, (T*)out, means, rstds);
     });
   };
-  const bool done = whole_packs<T>(a.channels, address(x) | address(out))
-                        ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
-                        : with_packs(std::integral_constant<int, 1>());
+  const bool done = packs ? with_packs(std::integral_constant<int, 16 / (int)sizeof(T)>())
+                          : with_packs(std::integral_constant<int, 1>());
   if (!done)
     hipLaunchKernelGGL((wide_norm_kernel<T, ENCODE>), dim3(nrows < 4096 ? nrows : 4096),
                        dim3(kThreads), 0, stream, (const T*)x, t, scale, a, bias, drop, (T*)out,

@@ -15,12 +15,15 @@ def test_case(name):
     assert p.returncode == 0 and name + " passed" in p.stdout, p.stdout[-3000:]
 
 
-def test_views_on_the_emulated_device():
+@pytest.mark.parametrize("name,passed", [("views", 2), ("rounds", 19)])
+def test_device_tests_on_the_emulated_device(name, passed):
+    """What the device tests ask of the functions; times and what needs autograd are left to the device."""
     here = os.path.dirname(RUNNER)
     p = subprocess.run([sys.executable, os.path.join(here, "gpu_tests_on_fake_device.py"),
-                        os.path.join(os.path.dirname(here), "test_type_vector_views_gpu.py"), "-m", "gpu", "-q"],
-                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=600)
-    assert p.returncode == 0 and "2 passed" in p.stdout, p.stdout[-3000:]
+                        os.path.join(os.path.dirname(here), "test_type_vector_%s_gpu.py" % name), "-m", "gpu", "-q",
+                        "-k", "not time"],
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=1200)
+    assert p.returncode == 0 and "%d passed" % passed in p.stdout, p.stdout[-3000:]
 
 
 def test_the_contracting_build_fuses_products_and_sums():
