@@ -104,7 +104,7 @@ int check_norm(const NormArg& a) {
   if (a.channels > kMaxVectorChannels) return MG_ERR_UNSUPPORTED;
   if (!is_dtype(a.dtype) || (a.param_dtype != MG_FLOAT32 && a.param_dtype != a.dtype))
     return MG_ERR_INVALID_ARGUMENT;
-  if (!(a.eps >= 0.f)) return MG_ERR_INVALID_ARGUMENT;
+  if (!(a.eps >= 0.f && std::isfinite(a.eps))) return MG_ERR_INVALID_ARGUMENT;
   if (!aligned(a.weight, dtype_size(a.param_dtype))) return MG_ERR_INVALID_ARGUMENT;
   return MG_OK;
 }
