@@ -46,9 +46,11 @@ __device__ __forceinline__ Stats wide_row_stats(const T* x, int channels, float 
 // Forward: a team holds a row in registers, sums it and its squared differences and writes it once.
 // The workgroups stay (kResident of them) and go through the rows, so that a lane reads its share of
 // weight and bias once; the next row's loads are in flight while a row is summed.
-// 32,768 x 8,192 bfloat16: 199 us (1.07 GB, 5.4 TB/s, what a copy reaches); 121,231 x 28 floats: 7.6 us.
+// 32,768 x 8,192 bfloat16: 201 us (1.07 GB, 5.3 TB/s; a copy of as much reaches 5.1); 121,231 x 28
+// floats: 7.7 us; 32,768 x 2,048 bfloat16 off a 16-byte boundary, an element a load: 93 us.
 // ENCODE: the rows are those of a scaled table, by the tokens' indices, and are dropped out.  32,768 x
-// 2,048 bfloat16: 57 us, bound by arithmetic (the generator's 20 wide products a pack are half of it).
+// 2,048 bfloat16: 50 to 55 us, 44 where nothing is dropped.  Its 22 million vector instructions, 8 million of
+// them the generator's, take 36 us to issue at 2.4 GHz.
 constexpr int kResident = 2048;
 
 template <typename T, int VEC, int LANES, int K, bool ENCODE>
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void few_rows_encode_kernel(
 }
 
 // Rows wider than any team (more than 8,192 channels): a workgroup goes over the row three times,
-// which stays in the caches.
+// which stays in the caches, an element a load: 8,192 x 12,288 bfloat16 in 255 us (1.6 TB/s).
 template <typename T, bool ENCODE>
 __global__ __launch_bounds__(kThreads) void wide_norm_kernel(const T* x, TokenArg tokens,
                                                              float scale, NormArg a,
@@ -271,8 +273,8 @@ __device__ __forceinline__ bool is_named(const NamedRows& named, uint32_t word, 
 }
 
 // Backward: a team holds the rows of x and of the gradient, writes dx, and a lane adds its share of
-// dw and db up over all rows that its team takes.  32,768 x 8,192 bfloat16: 325 us (1.6 GB, 5.0 TB/s) and
-// 8 us for the partial sums; 121,231 x 28 floats: 10 and 5 us.  G: type of the gradient; TABLE: x is a scaled
+// dw and db up over all rows that its team takes.  32,768 x 8,192 bfloat16: 329 us (1.6 GB, 4.9 TB/s) and
+// 8 us for the partial sums; 121,231 x 28 floats: 10 and 6 us.  G: type of the gradient; TABLE: x is a scaled
 // table, whose statistics are computed here.
 constexpr int kParts = 512, kNarrowParts = 1024;   // workgroups that share the rows
 
@@ -364,7 +366,8 @@ __global__ __launch_bounds__((TeamShape<LANES, K>::THREADS)) void norm_backward_
   if (to_params) add_up_params<T, VEC, LANES, K>(dw, db, lane, channels, sums, params);
 }
 
-// The same for rows wider than any team: dx, a workgroup a row, and dw and db, a thread a channel.
+// The same for rows wider than any team: dx, a workgroup a row, and dw and db, a thread a channel, which
+// are kept in the workgroup's row of partial sums: 8,192 x 12,288 bfloat16 in 243 and 1,085 us.
 template <typename T, typename G>
 __global__ __launch_bounds__(kThreads) void wide_norm_backward_kernel(
     const G* __restrict__ grad, const T* __restrict__ x, float scale, NormArg a, const float* means,
@@ -452,9 +455,9 @@ hipError_t sum_partials(const float* partial, int parts, int channels, void* gra
   return hipGetLastError();
 }
 
-// The encoder's rows are bound by arithmetic (the generator alone is half of it), so as many elements
-// a lane as go: what is done once a row (a division and a square root, the sums over the lanes) is
-// then shared by more of them: 2,048 channels of bfloat16 by 64 lanes 57 us, by 256 lanes 65 us.
+// The encoder's rows take more arithmetic than a norm's, so as many elements a lane as go: what is done
+// once a row (a division and a square root, the sums over the lanes) is then shared by more of them:
+// 2,048 channels of bfloat16 by 64 lanes 57 us, by 256 lanes 65 us.
 template <int VEC, bool ENCODE, typename F>
 bool with_norm_team(int packs, F f) {
   if constexpr (ENCODE && VEC == 8)

@@ -26,8 +26,8 @@ struct NormArg {
 // Which elements a call drops.  Element e of the flattened array takes half e % 8 (low half of a
 // word first) of the words of counter (e / 8, offset) under key seed, and is kept where that half
 // is at least `limit`; `factor` multiplies what is kept.  16 bits an element: one counter serves
-// eight of them, so that the generator (about 500 cycles a wave and counter) stays behind the
-// memory it runs beside; with 32 bits an element it would be the bound for 16-bit types.
+// eight of them, so that the generator (about 60 vector instructions a wave and counter, counted in
+// the encoder) stays behind the memory that dropout runs beside.
 struct DropArg {
   uint32_t limit;         // round(65536 p): 0 keeps everything, 65536 nothing
   float factor;           // 65536 / (65536 - limit), 0 when nothing is kept
